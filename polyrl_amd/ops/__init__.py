@@ -15,6 +15,9 @@ import torch
 
 from . import ref
 from . import seq  # noqa: F401  (sequence-mixer ops of the hybrid decoders)
+from .adapters import AdapterPlan, adapter_add, adapter_plan  # noqa: F401
+from .rules import (LogitRules, adjust_logits, append_tokens,  # noqa: F401
+                    token_words)
 
 _EXT = None
 _EXT_ERR: Optional[str] = None
@@ -452,6 +455,38 @@ def gather_logprobs_train(logits: torch.Tensor, labels: torch.Tensor
                           ) -> torch.Tensor:
     """(N, V) bf16 contiguous + (N,) int64 -> (N,) fp32, differentiable."""
     return _GatherLogprobsTrain.apply(logits.contiguous(), labels.long())
+
+
+class _DropoutTrain(torch.autograd.Function):
+    """Seeded dropout; the way back makes the same mask again (dropout.hip)."""
+
+    @staticmethod
+    def forward(ctx, x, drop, seed):
+        ctx.save_for_backward(seed)
+        ctx.drop = drop
+        if x.is_cuda:
+            return _require_ext().dropout(_in_words(x), drop, seed)
+        return ref.dropout(x, drop, seed)
+
+    @staticmethod
+    def backward(ctx, dy):
+        seed, = ctx.saved_tensors
+        return _DropoutTrain.apply(dy, ctx.drop, seed), None, None
+
+
+def dropout_train(x: torch.Tensor, p: float, seed: torch.Tensor
+                  ) -> torch.Tensor:
+    """Differentiable dropout of x (bf16, fp16 or fp32): elements become 0 with
+    probability p, in 65536ths, and x / (1 - p) otherwise.  What stays is a function of the
+    seed, (1,) int64 on x's device, and an element's place in x, the same on every
+    device; no mask is kept between the passes.  Another seed for every call."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout_train: p {p}")
+    if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != x.device:
+        raise ValueError("dropout_train: seed (1,) int64 on x's device")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("dropout_train: bf16, fp16 or fp32")
+    return _DropoutTrain.apply(x, round(p * 65536), seed)
 
 
 class _RopeTrain(torch.autograd.Function):

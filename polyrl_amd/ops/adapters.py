@@ -1,0 +1,81 @@
+"""Low-rank adapters of many requests beside a shared projection (adapters.hip).
+
+One step of a model groups its rows once (:func:`adapter_plan`) and then adds the
+adapters' part to each projection (:func:`adapter_add`).
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+from . import ref
+
+MOST_ADAPTERS = 4095
+MOST_PARTS = 8
+
+
+class AdapterPlan:
+    """Rows of a step by their adapters.  On the GPU the grouping is a tensor that
+    :func:`adapter_plan` computed there: calls wait for nothing and can be captured."""
+
+    def __init__(self, index: torch.Tensor, slots: int,
+                 table: Optional[torch.Tensor]):
+        self.index = index
+        self.slots = slots
+        self.table = table
+
+    @property
+    def rows(self) -> int:
+        return self.index.shape[0]
+
+
+def adapter_plan(index: torch.Tensor, slots: int) -> AdapterPlan:
+    """index (T,) int32: every row's adapter; one outside of 0 .. slots - 1 names none."""
+    if index.dim() != 1 or index.dtype != torch.int32:
+        raise ValueError("adapter_plan: index (T,) int32")
+    if not 1 <= slots <= MOST_ADAPTERS:
+        raise ValueError(f"adapter_plan: 1 to {MOST_ADAPTERS} adapters")
+    table = None
+    if index.is_cuda:
+        from . import _require_ext
+        index = index.contiguous()
+        table = _require_ext().adapter_plan(index, slots)
+    return AdapterPlan(index, slots, table)
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
+                b: torch.Tensor, scale: torch.Tensor, plan: AdapterPlan,
+                widths: Optional[Sequence[int]] = None,
+                ranks: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] + scale[i] * B_i (A_i x[t]) for the adapter i of every row, y[t] where a row
+    has none (no autograd).
+
+    y (T, N), x (T, K) rows of a projection's output and input; a (S, P, r, K) and b
+    (S, N, r): the S adapters of a projection of P parts whose ``widths`` add up to N
+    (q, k and v of one fused product; default: one part).  scale (S,) fp32.  ranks (S,)
+    int32: how much of r an adapter uses (0: none, its rows are y's); what a and b hold
+    beyond is not read.  ``out``: where the result goes, ``out=y`` in place.  bf16 or
+    fp32, all of one type."""
+    widths = [y.shape[1]] if widths is None else [int(w) for w in widths]
+    if torch.is_grad_enabled() and any(
+            t.requires_grad for t in (y, x, a, b, scale)):
+        raise RuntimeError("adapter_add has no gradients: call it under "
+                           "torch.no_grad()")
+    if plan.rows != y.shape[0]:
+        raise ValueError(f"adapter_add: a plan of {plan.rows} rows for "
+                         f"{y.shape[0]}")
+    if y.is_cuda:
+        from . import _NONE, _require_ext
+        ext = _require_ext()
+        if out is None:
+            out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        ext.adapter_add(out, y, x, a, b, scale,
+                        _NONE if ranks is None else ranks, plan.table,
+                        plan.slots, widths)
+        return out
+    res = ref.adapter_add(y, x, a, b, scale, plan.index, widths, ranks)
+    if out is None:
+        return res
+    return out.copy_(res)

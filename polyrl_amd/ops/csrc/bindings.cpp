@@ -92,6 +92,19 @@ torch::Tensor tuned_linear_dgrad(torch::Tensor dy, torch::Tensor w);
 torch::Tensor tuned_linear_wgrad(torch::Tensor dy, torch::Tensor x);
 torch::Tensor linear_wgrad(torch::Tensor dy, torch::Tensor x);
 torch::Tensor linear_dgrad(torch::Tensor dy, torch::Tensor w);
+torch::Tensor dropout(torch::Tensor x, int64_t drop, torch::Tensor seed);
+void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
+                   torch::Tensor history, torch::Tensor prompt_len,
+                   torch::Tensor total_len, torch::Tensor repetition,
+                   torch::Tensor frequency, torch::Tensor presence,
+                   torch::Tensor bias_tokens, torch::Tensor bias_values,
+                   torch::Tensor mask, torch::Tensor masked);
+void append_tokens(torch::Tensor history, torch::Tensor total_len, torch::Tensor rows,
+                   torch::Tensor tokens);
+torch::Tensor adapter_plan(torch::Tensor index, int64_t slots);
+void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Tensor a,
+                 torch::Tensor b, torch::Tensor scale, torch::Tensor ranks,
+                 torch::Tensor plan, int64_t slots, std::vector<int64_t> widths);
 void varlen_attention_backward_v3(
     torch::Tensor dq, torch::Tensor dk, torch::Tensor dv,
     torch::Tensor q, torch::Tensor k, torch::Tensor v,
@@ -161,6 +174,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "dW = dY^T X: the kernel for many rows, else algo-pinned");
   m.def("linear_wgrad", &linear_wgrad, "dW = dY^T X, the kernel");
   m.def("linear_dgrad", &linear_dgrad, "dX = dY W, the kernel");
+  m.def("dropout", &dropout, "seeded dropout, the mask from a counter-based generator");
+  m.def("adjust_logits", &adjust_logits,
+        "penalties, biases and allowed tokens on a step's logits");
+  m.def("append_tokens", &append_tokens, "tokens at the ends of histories");
+  m.def("adapter_plan", &adapter_plan, "rows in tiles of one adapter each");
+  m.def("adapter_add", &adapter_add, "y + s B (A x) by each row's adapter");
   m.def("varlen_attention_backward_v3", &varlen_attention_backward_v3,
         "varlen flash-attention backward v3 (atomic-free dkv+dq split, "
         "head_dim 64/128)");

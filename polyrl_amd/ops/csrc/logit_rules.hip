@@ -1,0 +1,257 @@
+// Rules of a request on its next token's logits, and the tokens that they go by.
+//
+//   u   = seen in prompt or output ? (l > 0 ? l / repetition : l * repetition) : l
+//   out = allowed ? u - frequency * c - presence * [c > 0] + bias : -inf
+// with c the token's times in the output so far.  Computed in 32 bits, rounded once to
+// the logits' type.
+//
+// Split.  No table of counts is kept per request (a row of 128256 would be as long as
+// its logits, read at every token and copied with every fork): the history itself is the
+// state.  A block takes ``chunk`` tokens of one row, counts the part of the history that
+// falls into them in LDS (a word per token: times said, seen, its bias), and passes
+// over the logits once.
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+#include "vocab_row.h"
+
+// a token's word in LDS
+constexpr uint32_t SAID = (1u << 19) - 1;   // times in the output
+constexpr uint32_t SEEN = 1u << 19;         // in the prompt
+constexpr int BIAS = 20;                    // from here: place in the biases + 1
+constexpr long MOST_TOKENS = SAID, MOST_BIASES = (1 << 12) - 1;
+
+struct Rules {
+  const int* rows;
+  const int* history;
+  const int* prompt_len;
+  const int* total_len;
+  const float *repetition, *frequency, *presence;
+  const int* bias_tokens;
+  const float* bias_values;
+  const int* mask;
+  const int* masked;
+  int slots, cap, biases, words;
+};
+
+// one rounding for each operation: the sums are the definition's
+DEV_INLINE float ruled(float l, uint32_t w, float rep, float freq, float pres,
+                       const float* __restrict__ values) {
+  const uint32_t c = w & SAID;
+  if (w & (SAID | SEEN)) l = l > 0.f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
+  if (c) l = __fsub_rn(__fsub_rn(l, __fmul_rn(freq, (float)c)), pres);
+  if (w >> BIAS) l = __fadd_rn(l, values[(w >> BIAS) - 1]);
+  return l;
+}
+
+template <typename T> DEV_INLINE T rounded(float x);
+template <> DEV_INLINE float rounded<float>(float x) { return x; }
+template <> DEV_INLINE bf16_t rounded<bf16_t>(float x) { return f2bf(x); }
+
+// WIDE: a row of logits and its row of out start at the same place of a 16-byte word
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void logit_rules_kernel(
+    T* out, const T* logits, const Rules a, int V, long ld, long ld_out, int chunk,
+    int chunks) {
+  constexpr int VEC = WIDE ? VocabRow<T>::VEC : 1;
+  extern __shared__ uint32_t lds[];
+  const long row = blockIdx.x / chunks;
+  const int part = blockIdx.x % chunks, tid = threadIdx.x;
+  const int slot = a.rows[row];
+  const bool ruled_row = slot >= 0 && slot < a.slots;
+  const VocabRow<T> in(logits + row * ld, V);
+  T* to = out + row * ld_out;
+  // groups of VEC tokens; the first one of a row that starts inside a word is short
+  const int lead = WIDE ? in.lead : 0, ahead = WIDE ? 1 : 0;
+  const int all = ahead + (V - lead + VEC - 1) / VEC;
+  const int g0 = part * (chunk / VEC), g1 = min(g0 + chunk / VEC, all);
+  const int base = lead + (g0 - ahead) * VEC;     // token of LDS word 0, may be < 0
+  const bool same = out == logits;
+  float rep = 1.f, freq = 0.f, pres = 0.f;
+  bool counts = false, biased = false, masked = false;
+  int total = 0, prompt = 0;
+  if (ruled_row) {
+    rep = a.repetition[slot], freq = a.frequency[slot], pres = a.presence[slot];
+    total = min(max(a.total_len[slot], 0), a.cap);
+    prompt = min(max(a.prompt_len[slot], 0), total);
+    counts = total > 0 && (rep != 1.f || freq != 0.f || pres != 0.f);
+    biased = a.biases > 0;
+    masked = a.masked[slot] != 0;
+  }
+  if (same && !counts && !biased && !masked) return;
+  const float* values = a.bias_values + (long)slot * a.biases;
+  if (counts || biased) {
+    for (int i = tid; i < chunk; i += 256) lds[i] = 0;
+    __syncthreads();
+    if (counts) {
+      const int* h = a.history + (long)slot * a.cap;
+      for (int i = tid; i < total; i += 256) {
+        const int t = h[i] - base;
+        if ((unsigned)t < (unsigned)chunk && h[i] >= 0) {
+          if (i < prompt) atomicOr(&lds[t], SEEN);
+          else atomicAdd(&lds[t], 1u);
+        }
+      }
+      __syncthreads();
+    }
+    // the last entry of a token holds; the lower bits stand still by now
+    if (biased) {
+      const int* b = a.bias_tokens + (long)slot * a.biases;
+      for (int i = tid; i < a.biases; i += 256) {
+        const int t = b[i] - base;
+        if ((unsigned)t < (unsigned)chunk && b[i] >= 0)
+          atomicMax(&lds[t], (uint32_t)(i + 1) << BIAS |
+                                 (lds[t] & ((1u << BIAS) - 1)));
+      }
+      __syncthreads();
+    }
+  }
+  const int* mask = a.mask + (long)slot * a.words;
+  for (int g = g0 + tid; g < g1; g += 256) {
+    const int i0 = lead + (g - ahead) * VEC;
+    uint32_t w[VEC], any = 0;
+    if (counts || biased) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) any |= w[j] = lds[i0 - base + j];
+    }
+    if (same && !masked && any == 0) continue;
+    float v[VEC];
+    if (WIDE) {
+      float u[VocabRow<T>::VEC];
+      in.load(g, u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = u[j];
+    } else {
+      v[0] = (float)in.x[i0];
+    }
+    if (any != 0) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = ruled(v[j], w[j], rep, freq, pres, values);
+    }
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const int i = i0 + j;
+        if (i >= 0 && i < V && !(mask[i >> 5] >> (i & 31) & 1)) v[j] = -INFINITY;
+      }
+    }
+    if (WIDE && i0 >= 0 && i0 + VEC <= V) {
+      struct alignas(16) Vec { T v[VEC]; } o;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o.v[j] = rounded<T>(v[j]);
+      *reinterpret_cast<Vec*>(to + i0) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (i0 + j >= 0 && i0 + j < V) to[i0 + j] = rounded<T>(v[j]);
+    }
+  }
+}
+
+// Tokens at the ends of their slots' histories: row i's behind those of the rows
+// before it with the same slot.  One block
+__global__ __launch_bounds__(256) void append_tokens_kernel(
+    int* history, int* total_len, const int* rows, const int64_t* tokens, int N,
+    int slots, int cap) {
+  for (int step = 0; step < 2; ++step) {
+    for (int i = threadIdx.x; i < N; i += 256) {
+      const int s = rows[i];
+      if (s < 0 || s >= slots) continue;
+      int before = 0, behind = 0;
+      for (int j = 0; j < N; ++j)
+        if (rows[j] == s) j < i ? ++before : j > i ? ++behind : 0;
+      const long at = (long)min(max(total_len[s], 0), cap) + before;
+      if (step == 0) {
+        const int64_t t = tokens[i];
+        if (at < cap) history[(long)s * cap + at] = t >= 0 && t < (1L << 31) ? (int)t : -1;
+      } else if (behind == 0) {
+        total_len[s] = (int)min(at + 1, (long)cap);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+static void check_ints(const torch::Tensor& t, const torch::Tensor& by, const char* what) {
+  TORCH_CHECK(t.device() == by.device() && t.scalar_type() == torch::kInt32 &&
+                  t.is_contiguous(),
+              what, ": contiguous int32 on the same device");
+}
+
+void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
+                   torch::Tensor history, torch::Tensor prompt_len,
+                   torch::Tensor total_len, torch::Tensor repetition,
+                   torch::Tensor frequency, torch::Tensor presence,
+                   torch::Tensor bias_tokens, torch::Tensor bias_values,
+                   torch::Tensor mask, torch::Tensor masked) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && out.sizes() == logits.sizes() &&
+                  out.device() == logits.device() &&
+                  out.scalar_type() == logits.scalar_type(),
+              "adjust_logits: logits and out (N, V) of one type and device");
+  const long N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK((V <= 1 || (logits.stride(1) == 1 && out.stride(1) == 1)) &&
+                  V < (1L << 30),
+              "adjust_logits: rows of adjacent numbers");
+  for (const auto& t : {rows, history, prompt_len, total_len, bias_tokens, mask, masked})
+    check_ints(t, logits, "adjust_logits");
+  const long R = history.size(0), cap = history.size(1), nb = bias_tokens.size(1);
+  TORCH_CHECK(rows.dim() == 1 && rows.size(0) == N && prompt_len.numel() == R &&
+                  total_len.numel() == R && masked.numel() == R && mask.size(0) == R &&
+                  mask.size(1) == (V + 31) / 32 && bias_tokens.size(0) == R &&
+                  bias_values.sizes() == bias_tokens.sizes(),
+              "adjust_logits: rules of another shape");
+  for (const auto& t : {repetition, frequency, presence, bias_values})
+    TORCH_CHECK(t.device() == logits.device() && t.scalar_type() == torch::kFloat32 &&
+                    t.is_contiguous() && (t.dim() == 2 || t.numel() == R),
+                "adjust_logits: contiguous fp32 rules");
+  TORCH_CHECK(cap <= MOST_TOKENS && nb <= MOST_BIASES, "adjust_logits: at most ",
+              MOST_TOKENS, " tokens and ", MOST_BIASES, " biases a slot");
+  if (N == 0 || V == 0) return;
+  const c10::DeviceGuard guard(logits.device());
+  const Rules a{rows.data_ptr<int>(), history.data_ptr<int>(),
+                prompt_len.data_ptr<int>(), total_len.data_ptr<int>(),
+                repetition.data_ptr<float>(), frequency.data_ptr<float>(),
+                presence.data_ptr<float>(), bias_tokens.data_ptr<int>(),
+                bias_values.data_ptr<float>(), mask.data_ptr<int>(),
+                masked.data_ptr<int>(), (int)R, (int)cap, (int)nb, (int)mask.size(1)};
+  int chunk = 8192;
+  while (chunk > 1024 && N * ((V + chunk - 1) / chunk) < 512) chunk /= 2;
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const uintptr_t at = (uintptr_t)logits.data_ptr() ^ (uintptr_t)out.data_ptr();
+    const bool wide = (at & 15) == 0 &&
+                      ((logits.stride(0) - out.stride(0)) * sizeof(T) & 15) == 0;
+    // (a row that starts inside a word has one group more)
+    const long chunks = (V + (wide ? 16 / (long)sizeof(T) : 0) + chunk - 1) / chunk;
+    TORCH_CHECK(N * chunks < (1L << 31), "adjust_logits: too many rows");
+    auto kern = wide ? logit_rules_kernel<T, true> : logit_rules_kernel<T, false>;
+    kern<<<dim3((unsigned)(N * chunks)), dim3(256), chunk * 4,
+           at::hip::getCurrentHIPStream()>>>(
+        (T*)out.data_ptr(), (const T*)logits.data_ptr(), a, (int)V, logits.stride(0),
+        out.stride(0), chunk, (int)chunks);
+  };
+  if (logits.scalar_type() == torch::kBFloat16) go(bf16_t{});
+  else if (logits.scalar_type() == torch::kFloat32) go(float{});
+  else TORCH_CHECK(false, "adjust_logits: dtype must be bf16 or fp32");
+  HIP_CHECK_KERNEL();
+}
+
+void append_tokens(torch::Tensor history, torch::Tensor total_len, torch::Tensor rows,
+                   torch::Tensor tokens) {
+  TORCH_CHECK(history.is_cuda() && history.dim() == 2 && rows.dim() == 1 &&
+                  total_len.numel() == history.size(0),
+              "append_tokens: history (slots, capacity), rows (N)");
+  for (const auto& t : {history, total_len, rows}) check_ints(t, history, "append_tokens");
+  TORCH_CHECK(tokens.device() == history.device() && tokens.is_contiguous() &&
+                  tokens.scalar_type() == torch::kInt64 && tokens.numel() == rows.numel(),
+              "append_tokens: tokens (N) int64");
+  TORCH_CHECK(rows.numel() <= 65536, "append_tokens: at most 65536 rows");
+  if (rows.numel() == 0) return;
+  const c10::DeviceGuard guard(history.device());
+  append_tokens_kernel<<<dim3(1), dim3(256), 0, at::hip::getCurrentHIPStream()>>>(
+      history.data_ptr<int>(), total_len.data_ptr<int>(), rows.data_ptr<int>(),
+      tokens.data_ptr<int64_t>(), (int)rows.numel(), (int)history.size(0),
+      (int)history.size(1));
+  HIP_CHECK_KERNEL();
+}

@@ -203,3 +203,102 @@ def varlen_lse(q, k, cu_seqlens_q, cu_seqlens_k, scale, causal=True):
                 s = s.masked_fill(kpos > qpos, float("-inf"))
             out[q0:q1, h] = torch.logsumexp(s, dim=-1)
     return out
+
+
+# ------------------------------------------------------- adapters of requests
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
+                b: torch.Tensor, scale: torch.Tensor, index: torch.Tensor,
+                widths, ranks: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y + scale[i] * B_i (A_i x) by every row's adapter i = index[t]; rows without one
+    are y's.  a (S, P, r, K), b (S, N, r), parts of ``widths`` columns."""
+    S, P, r, K = a.shape
+    if (x.shape != (y.shape[0], K) or b.shape != (S, y.shape[1], r)
+            or len(widths) != P or sum(widths) != y.shape[1]):
+        raise ValueError("adapter_add: shapes that do not fit together")
+    out = y.clone()
+    for s in range(S):
+        rows = (index == s).nonzero().flatten()
+        n = r if ranks is None else min(max(int(ranks[s]), 0), r)
+        if not len(rows) or n == 0:
+            continue
+        total = y[rows].float()
+        at = 0
+        for p, w in enumerate(widths):
+            h = x[rows].float() @ a[s, p, :n].float().t() * scale[s]
+            total[:, at:at + w] += h @ b[s, at:at + w, :n].float().t()
+            at += w
+        out[rows] = total.to(y.dtype)
+    return out
+
+
+# ------------------------------------------------------------ rules on logits
+
+
+def adjust_logits(logits: torch.Tensor, rules, rows: torch.Tensor
+                  ) -> torch.Tensor:
+    out = logits.clone()
+    V = logits.shape[1]
+    for i, s in enumerate(rows.tolist()):
+        if not 0 <= s < rules.slots:
+            continue
+        total = min(max(int(rules.total_len[s]), 0), rules.capacity)
+        prompt = min(max(int(rules.prompt_len[s]), 0), total)
+        words = rules.history[s, :total].long()
+        known = (words >= 0) & (words < V)
+        asked, said = (torch.bincount(w[k], minlength=V) for w, k in (
+            (words[:prompt], known[:prompt]), (words[prompt:], known[prompt:])))
+        x = logits[i].float()
+        rep = rules.repetition[s]
+        x = torch.where(asked + said > 0, torch.where(x > 0, x / rep, x * rep), x)
+        x = torch.where(said > 0, x - rules.frequency[s] * said.float()
+                        - rules.presence[s], x)
+        last = {t: v for t, v in zip(rules.bias_tokens[s].tolist(),
+                                     rules.bias_values[s].tolist())
+                if 0 <= t < V}
+        if last:
+            x[list(last)] += torch.tensor(list(last.values()))
+        if rules.masked[s]:
+            words = rules.mask[s].unsqueeze(1) >> torch.arange(32)
+            x = x.masked_fill((words & 1).flatten()[:V] == 0, float("-inf"))
+        out[i] = x.to(logits.dtype)
+    return out
+
+
+def append_tokens(rules, rows: torch.Tensor, tokens: torch.Tensor) -> None:
+    for s, t in zip(rows.tolist(), tokens.tolist()):
+        if not 0 <= s < rules.slots:
+            continue
+        at = max(int(rules.total_len[s]), 0)
+        if at < rules.capacity:
+            rules.history[s, at] = t if 0 <= t < 1 << 31 else -1
+            rules.total_len[s] = at + 1
+
+
+# ------------------------------------------------------------- seeded dropout
+
+
+def dropout_keep(numel: int, drop: int, seed: int) -> torch.Tensor:
+    """Whether each of ``numel`` elements stays: Philox4x32-10 (Salmon, Moraes, Dror and
+    Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011), eight numbers of 16
+    bits for every counter, key = seed."""
+    low = (1 << 32) - 1
+    at = torch.arange((numel + 7) // 8)
+    zero = torch.zeros_like(at)
+    c = [at & low, at >> 32, zero, zero]
+    key = [seed & low, (seed >> 32) & low]
+    for _ in range(10):
+        p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [((q >> 32) & low) ^ c[1] ^ key[0], q & low,
+             ((p >> 32) & low) ^ c[3] ^ key[1], p & low]
+        key = [(key[0] + 0x9E3779B9) & low, (key[1] + 0xBB67AE85) & low]
+    words = torch.stack(c, -1)
+    return torch.stack([words & 0xffff, words >> 16], -1).flatten()[:numel] >= drop
+
+
+def dropout(x: torch.Tensor, drop: int, seed: torch.Tensor) -> torch.Tensor:
+    """Elements that stay, times 65536 / (65536 - drop); zeros for the others."""
+    keep = dropout_keep(x.numel(), drop, int(seed)).view(x.shape)
+    scale = 65536.0 / (65536 - drop) if drop < 65536 else 0.0
+    return torch.where(keep, x.float() * scale, 0.0).to(x.dtype)

@@ -1,0 +1,270 @@
+"""Low-rank adapters of many requests beside a shared projection, against 64 bits."""
+import pytest
+import torch
+
+import polyrl_amd.ops as ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def make(dev, dtype, T, K, widths, r, S, seed=0, pad=0, shift=0):
+    """y, x, a, b, scale; rows ``pad`` numbers longer than they are and ``shift``
+    numbers into their memory."""
+    g = torch.Generator().manual_seed(seed)
+
+    def rows(n, width):
+        full = torch.randn(n * (width + pad) + shift, generator=g).to(dtype).to(dev)
+        return full[shift:].view(n, width + pad)[:, :width]
+    N = sum(widths)
+    a = (torch.randn(S, len(widths), r, K, generator=g) * K ** -0.5).to(dtype).to(dev)
+    b = torch.randn(S, N, r, generator=g).to(dtype).to(dev)
+    scale = (torch.rand(S, generator=g) + 0.5).to(dev)
+    return rows(T, N), rows(T, K), a, b, scale
+
+
+def expected(y, x, a, b, scale, index, widths, ranks=None):
+    """The result and how far off it may be.
+
+    h = A x is a sum of K products in 32 bits, then split into two bf16 numbers for
+    bf16 (2^-8 of what 2^-8 leaves); B h a sum of r products in 32 bits, of hi and lo
+    apart; y is added in 32 bits and the sum rounded once."""
+    y, x, a, b = (t.double().cpu() for t in (y, x, a, b))
+    S, P, r, K = a.shape
+    want, size = y.clone(), torch.zeros_like(y)
+    for t, s in enumerate(index.tolist()):
+        if not 0 <= s < S:
+            continue
+        n = r if ranks is None else int(ranks[s])
+        at = 0
+        for p, w in enumerate(widths):
+            A, B = a[s, p, :n], b[s, at:at + w, :n]
+            want[t, at:at + w] += float(scale[s]) * (B @ (A @ x[t]))
+            size[t, at:at + w] += float(scale[s]) * (B.abs() @ (A.abs() @ x[t].abs()))
+            at += w
+    return want, size
+
+
+def close(got, want, size, y, K, r):
+    eps = torch.finfo(got.dtype).eps / 2
+    lost = 2.0 ** -16 if got.dtype == BF16 else 0.0
+    inner = size * ((K + 2 * r + 32) * 2.0 ** -24 + lost)
+    inner = inner + 2.0 ** -23 * (y.double().cpu().abs() + size)
+    diff = (got.double().cpu() - want).abs()
+    bad = diff > eps * (want.abs() + inner) + inner
+    assert not bad.any(), (diff.max(), bad.nonzero()[:5])
+
+
+SIZES = [
+    # T, K, widths, r, S
+    (1, 64, (16,), 1, 1),
+    (1, 1024, (1024, 256, 256), 8, 4),
+    (5, 33, (7,), 5, 3),
+    (16, 128, (48, 16, 7), 16, 2),
+    (17, 100, (64, 64), 33, 5),
+    (57, 256, (300,), 64, 70),
+    (257, 192, (256, 64, 64), 20, 3),
+    (300, 520, (130,), 100, 7),
+    (64, 4096, (32,), 16, 2),
+    (3, 1, (1,), 1, 1),
+]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", SIZES)
+def test_against_64_bits(dev, dtype, size):
+    T, K, widths, r, S = size
+    y, x, a, b, scale = make(dev, dtype, T, K, widths, r, S)
+    g = torch.Generator().manual_seed(1)
+    index = torch.randint(-1, S + 1, (T,), generator=g, dtype=torch.int32)
+    index[0] = 0
+    plan = ops.adapter_plan(index.to(dev), S)
+    keep = y.clone()
+    got = ops.adapter_add(y, x, a, b, scale, plan, widths)
+    assert torch.equal(y, keep)
+    want, size = expected(y, x, a, b, scale, index, widths)
+    close(got, want, size, y, K, r)
+    none = (index < 0) | (index >= S)
+    assert torch.equal(got[none.to(dev)], y[none.to(dev)])
+    # in place: the same bits
+    assert ops.adapter_add(y, x, a, b, scale, plan, widths, out=y) is y
+    assert torch.equal(y, got)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("pad,shift", [(8, 0), (3, 0), (0, 1), (5, 3)])
+@pytest.mark.parametrize("T", [9, 260])
+def test_strides_and_addresses(dev, dtype, pad, shift, T):
+    K, widths, r, S = 72, (40, 24), 16, 3
+    y, x, a, b, scale = make(dev, dtype, T, K, widths, r, S, pad=pad, shift=shift)
+    index = (torch.arange(T, dtype=torch.int32) % 4) - 1
+    around = y._base.clone()
+    plan = ops.adapter_plan(index.to(dev), S)
+    got = ops.adapter_add(y, x, a, b, scale, plan, widths)
+    want, size = expected(y, x, a, b, scale, index, widths)
+    close(got, want, size, y, K, r)
+    ops.adapter_add(y, x, a, b, scale, plan, widths, out=y)
+    assert torch.equal(y, got)
+    # what lies between and before the rows is as it was
+    after = y._base.clone()
+    mask = torch.ones_like(after, dtype=torch.bool)
+    mask[shift:].view(T, -1)[:, :sum(widths)] = False
+    assert torch.equal(after[mask], around[mask])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [40, 300])
+def test_ranks(dev, dtype, T):
+    """Smaller ranks in a pool: what lies beyond them is not read; rank 0 is none."""
+    K, widths, r, S = 128, (64, 32), 40, 6
+    y, x, a, b, scale = make(dev, dtype, T, K, widths, r, S)
+    ranks = torch.tensor([40, 0, 1, 16, 33, 7], dtype=torch.int32)
+    for s in range(S):
+        a[s, :, ranks[s]:] = float("nan")
+        b[s, :, ranks[s]:] = float("nan")
+    index = torch.arange(T, dtype=torch.int32) % S
+    plan = ops.adapter_plan(index.to(dev), S)
+    got = ops.adapter_add(y, x, a, b, scale, plan, widths, ranks=ranks.to(dev))
+    want, size = expected(y, x, a, b, scale, index, widths, ranks)
+    close(got, want, size, y, K, r)
+    assert torch.equal(got[index == 1], y[index == 1])
+    out = y.clone()
+    ops.adapter_add(out, x, a, b, scale, plan, widths, ranks=ranks.to(dev), out=out)
+    assert torch.equal(out, got)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_do_not_touch_each_other(dev, dtype):
+    """An infinite or undefined row stays its own, an infinite h stays infinite."""
+    T, K, r, S = 33, 64, 8, 2
+    y, x, a, b, scale = make(dev, dtype, T, K, (32,), r, S)
+    index = torch.arange(T, dtype=torch.int32) % S
+    plan = ops.adapter_plan(index.to(dev), S)
+    clean = ops.adapter_add(y, x, a, b, scale, plan)
+    x[4] = float("nan")
+    a[0, 0, 0], b[0, :, 0] = 1.0, 1.0
+    a[0, 0, 1:] = 0.0
+    clean0 = ops.adapter_add(y, x, a, b, scale, plan)
+    x[6] = torch.finfo(dtype).max               # sums to infinity
+    got = ops.adapter_add(y, x, a, b, scale, plan)
+    assert got[4].isnan().all()
+    assert (got[6] == float("inf")).all()
+    for t in range(T):
+        if t not in (4, 6):
+            assert torch.equal(got[t], (clean if index[t] else clean0)[t])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_none_and_empty(dev):
+    y, x, a, b, scale = make(dev, BF16, 20, 32, (16,), 8, 2)
+    for v in (-1, -7, 2, 99):
+        plan = ops.adapter_plan(torch.full((20,), v, dtype=torch.int32, device=dev), 2)
+        assert torch.equal(ops.adapter_add(y, x, a, b, scale, plan), y)
+    plan = ops.adapter_plan(torch.zeros(0, dtype=torch.int32, device=dev), 2)
+    assert ops.adapter_add(y[:0], x[:0], a, b, scale, plan).shape == (0, 16)
+
+
+@pytest.mark.gpu
+def test_many_rows_and_slots():
+    """Plans of many rows and of the most adapters, in any order."""
+    S, K, N, r = 4095, 64, 32, 4
+    y, x, a, b, scale = make("cuda", F32, 20000, K, (N,), r, S)
+    g = torch.Generator().manual_seed(3)
+    index = torch.randint(-1, S, (20000,), generator=g, dtype=torch.int32)
+    index[:9000] = 17
+    plan = ops.adapter_plan(index.cuda(), S)
+    got = ops.adapter_add(y, x, a, b, scale, plan)
+    i = index.clamp(min=0).long().cuda()
+    h = (a[i, 0].double() @ x.double().unsqueeze(-1))
+    d = (b[i].double() @ h).squeeze(-1) * scale[i].double().unsqueeze(1)
+    d[(index < 0).cuda()] = 0
+    h = (a[i, 0].double().abs() @ x.double().abs().unsqueeze(-1))
+    size = (b[i].double().abs() @ h).squeeze(-1) * scale[i].double().unsqueeze(1)
+    close(got, (y.double() + d).cpu(), size.cpu(), y, K, r)
+
+
+@pytest.mark.gpu
+def test_result_does_not_hang_on_the_order_of_rows():
+    T, K, widths, r, S = 600, 512, (96,), 24, 4
+    y, x, a, b, scale = make("cuda", BF16, T, K, widths, r, S)
+    g = torch.Generator().manual_seed(4)
+    index = torch.randint(-1, S, (T,), generator=g, dtype=torch.int32).cuda()
+    want = ops.adapter_add(y, x, a, b, scale, ops.adapter_plan(index, S))
+    for seed in range(3):
+        p = torch.randperm(T, generator=g).cuda()
+        got = ops.adapter_add(y[p], x[p], a, b, scale,
+                              ops.adapter_plan(index[p], S))
+        assert torch.equal(got, want[p])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 400])
+def test_captured(T):
+    """A captured step goes by the adapters of its replay."""
+    K, widths, r, S = 256, (64, 32), 16, 3
+    y, x, a, b, scale = make("cuda", BF16, T, K, widths, r, S)
+    index = torch.zeros(T, dtype=torch.int32, device="cuda")
+
+    def step():
+        plan = ops.adapter_plan(index, S)
+        return ops.adapter_add(y, x, a, b, scale, plan, widths)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    g = torch.Generator().manual_seed(5)
+    for _ in range(4):
+        index.copy_(torch.randint(-1, S + 1, (T,), generator=g))
+        x.copy_(torch.randn(T, K, generator=g))
+        graph.replay()
+        replayed = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, step())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals(dev):
+    y, x, a, b, scale = make(dev, BF16, 6, 32, (16,), 8, 2)
+    index = torch.zeros(6, dtype=torch.int32, device=dev)
+    plan = ops.adapter_plan(index, 2)
+    error = (ValueError, RuntimeError)
+    for bad in (index.long(), index.view(2, 3)):
+        with pytest.raises(error):
+            ops.adapter_plan(bad, 2)
+    for slots in (0, 4096):
+        with pytest.raises(error):
+            ops.adapter_plan(index, slots)
+    with pytest.raises(error):                              # another number of rows
+        ops.adapter_add(y[:5], x[:5], a, b, scale, plan)
+    with pytest.raises(error):
+        ops.adapter_add(y, x[:5], a, b, scale, plan)
+    for widths in ((8, 8), (8,), (16, 0)):
+        with pytest.raises(error):
+            ops.adapter_add(y, x, a, b, scale, plan, widths)
+    with pytest.raises(error):
+        ops.adapter_add(y, x[:, :31], a, b, scale, plan)
+    with pytest.raises(error):
+        ops.adapter_add(y, x, a, b[:, :15], scale, plan)
+    with pytest.raises(error):
+        ops.adapter_add(y, x, a.clone().requires_grad_(), b, scale, plan)
+    if dev == "cuda":
+        for bad in (x.float(), x.half()):
+            with pytest.raises(error):
+                ops.adapter_add(y, bad, a, b, scale, plan)
+        with pytest.raises(error):
+            ops.adapter_add(y.half(), x.half(), a.half(), b.half(), scale, plan)
+        with pytest.raises(error):
+            ops.adapter_add(y, x, a, b, scale.double(), plan)
+        with pytest.raises(error):
+            ops.adapter_add(y, x, a.cpu(), b, scale, plan)
+        with pytest.raises(error):                          # a plan of other adapters
+            ops.adapter_add(y, x, a[:1].contiguous(), b[:1].contiguous(), scale[:1],
+                            plan)
