@@ -458,14 +458,12 @@ def gather_logprobs_train(logits: torch.Tensor, labels: torch.Tensor
 
 
 class _DropoutTrain(torch.autograd.Function):
-    """Seeded dropout; the way back makes the same mask again (dropout.hip)."""
+    """Seeded dropout on the CPU; the way back makes the same mask again."""
 
     @staticmethod
     def forward(ctx, x, drop, seed):
         ctx.save_for_backward(seed)
         ctx.drop = drop
-        if x.is_cuda:
-            return _require_ext().dropout(_in_words(x), drop, seed)
         return ref.dropout(x, drop, seed)
 
     @staticmethod
@@ -486,7 +484,10 @@ def dropout_train(x: torch.Tensor, p: float, seed: torch.Tensor
         raise ValueError("dropout_train: seed (1,) int64 on x's device")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError("dropout_train: bf16, fp16 or fp32")
-    return _DropoutTrain.apply(x, round(p * 65536), seed)
+    drop = round(p * 65536)
+    if x.is_cuda:                  # an autograd function of dropout.hip
+        return _require_ext().dropout_train(x, drop, seed)
+    return _DropoutTrain.apply(x, drop, seed)
 
 
 class _RopeTrain(torch.autograd.Function):

@@ -92,7 +92,8 @@ torch::Tensor tuned_linear_dgrad(torch::Tensor dy, torch::Tensor w);
 torch::Tensor tuned_linear_wgrad(torch::Tensor dy, torch::Tensor x);
 torch::Tensor linear_wgrad(torch::Tensor dy, torch::Tensor x);
 torch::Tensor linear_dgrad(torch::Tensor dy, torch::Tensor w);
-torch::Tensor dropout(torch::Tensor x, int64_t drop, torch::Tensor seed);
+torch::Tensor dropout_train(const torch::Tensor& x, int64_t drop,
+                            const torch::Tensor& seed);
 void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
                    torch::Tensor history, torch::Tensor prompt_len,
                    torch::Tensor total_len, torch::Tensor repetition,
@@ -174,7 +175,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "dW = dY^T X: the kernel for many rows, else algo-pinned");
   m.def("linear_wgrad", &linear_wgrad, "dW = dY^T X, the kernel");
   m.def("linear_dgrad", &linear_dgrad, "dX = dY W, the kernel");
-  m.def("dropout", &dropout, "seeded dropout, the mask from a counter-based generator");
+  m.def("dropout_train", &dropout_train, "seeded dropout, differentiable, no mask kept");
   m.def("adjust_logits", &adjust_logits,
         "penalties, biases and allowed tokens on a step's logits");
   m.def("append_tokens", &append_tokens, "tokens at the ends of histories");

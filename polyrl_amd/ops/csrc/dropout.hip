@@ -7,6 +7,10 @@
 // elements.  Its four words are eight numbers of 16 bits; an element stays if its
 // number is at least ``drop`` = p in 65536ths, and is multiplied by
 // 65536 / (65536 - drop), so that the expectation is x whatever p was rounded to.
+//
+// What bounds it: memory (8192 x 14336 bf16, forward and backward, 175 us, 5.4 TB/s; 8192 x
+// 4096 53 us).  Of a group 20 products of 32 x 32 bits, at 16 cycles each, make its numbers; 32 bits
+// for each element would take twice as many, about the time that memory takes.
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -64,9 +68,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(
   }
 }
 
-torch::Tensor dropout(torch::Tensor x, int64_t drop, torch::Tensor seed) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && ((uintptr_t)x.data_ptr() & 15) == 0,
-              "dropout: contiguous x on the GPU at a 16-byte address");
+static torch::Tensor dropout(torch::Tensor x, int64_t drop, const torch::Tensor& seed) {
+  TORCH_CHECK(x.is_cuda(), "dropout: x on the GPU");
+  x = x.contiguous();
+  if ((uintptr_t)x.data_ptr() & 15) x = x.clone();
   TORCH_CHECK(seed.device() == x.device() && seed.scalar_type() == torch::kInt64 &&
                   seed.numel() == 1,
               "dropout: seed (1) int64 on x's device");
@@ -89,4 +94,27 @@ torch::Tensor dropout(torch::Tensor x, int64_t drop, torch::Tensor seed) {
   else TORCH_CHECK(false, "dropout: dtype must be bf16, fp16 or fp32");
   HIP_CHECK_KERNEL();
   return out;
+}
+
+// The way back makes the mask again, so that it is the same function of dy.  (In C++: a
+// small call and its gradient take 46 us, through Python's autograd functions 75; the
+// kernels take 5.)
+struct Dropout : torch::autograd::Function<Dropout> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx,
+                               const torch::Tensor& x, int64_t drop,
+                               const torch::Tensor& seed) {
+    ctx->save_for_backward({seed});
+    ctx->saved_data["drop"] = drop;
+    return dropout(x, drop, seed);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list dy) {
+    const auto seed = ctx->get_saved_variables()[0];
+    return {Dropout::apply(dy[0], ctx->saved_data["drop"].toInt(), seed), {}, {}};
+  }
+};
+
+torch::Tensor dropout_train(const torch::Tensor& x, int64_t drop,
+                            const torch::Tensor& seed) {
+  return Dropout::apply(x, drop, seed);
 }
