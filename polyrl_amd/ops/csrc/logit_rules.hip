@@ -7,14 +7,25 @@
 //
 // Split.  No table of counts is kept per request (a row of 128256 would be as long as
 // its logits, read at every token and copied with every fork): the history itself is the
-// state.  A block takes ``chunk`` tokens of one row, counts the part of the history that
-// falls into them in LDS (a word per token: times said, seen, its bias), and passes
-// over the logits once.
+// state.  A block takes a chunk of one row, counts the part of the history that falls into
+// it in LDS (a word per token: times said, seen, its bias), and passes over the logits once.
+//
+// What bounds it: memory, and before it the chain row -> slot -> history -> counts in each
+// block (128 x 128256 bf16, 257 to 512 tokens of history, 16 biases: 17.0 us, 3.9 TB/s, 12
+// without rules; 64 x 151936 fp32 with masks 17.6, 4.5 TB/s, what a copy takes).  Long
+// histories are read by every chunk of their row (33 x 152064, 9000 to 32768 tokens: 18.6).
+// What it took: 4-byte reads of the history, one waited for after the other 54 us of the
+// last, words 33; loads of the logits behind those of the history, so that a wait for
+// these does not wait for them, and barriers for LDS alone 19.9 -> 18.1 of the first; blocks of
+// 256 threads or chunks of four words a thread 20 to 24.  Bits for the tokens that the
+// counts touch, whose words alone are cleared, lose (20.5; 24.1 for 16.9 of the last).
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
 #include "vocab_row.h"
+
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
 // a token's word in LDS
 constexpr uint32_t SAID = (1u << 19) - 1;   // times in the output
@@ -49,29 +60,56 @@ template <typename T> DEV_INLINE T rounded(float x);
 template <> DEV_INLINE float rounded<float>(float x) { return x; }
 template <> DEV_INLINE bf16_t rounded<bf16_t>(float x) { return f2bf(x); }
 
-// WIDE: a row of logits and its row of out start at the same place of a 16-byte word
-template <typename T, bool WIDE>
-__global__ __launch_bounds__(256) void logit_rules_kernel(
-    T* out, const T* logits, const Rules a, int V, long ld, long ld_out, int chunk,
-    int chunks) {
-  constexpr int VEC = WIDE ? VocabRow<T>::VEC : 1;
-  extern __shared__ uint32_t lds[];
+constexpr int NT = 512;                     // threads of a block
+constexpr int HW = 2;                       // words of history that a thread has at a time
+
+// A barrier for what lies in LDS alone: loads from memory stay on their way
+DEV_INLINE void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A block takes NT * U words of VEC tokens of a row, each thread U of them, which are on
+// their way while the history is counted.  WIDE: a row of logits and its row of out start
+// at the same place of a 16-byte word
+template <typename T, bool WIDE, int U>
+__global__ __launch_bounds__(NT) void logit_rules_kernel(
+    T* out, const T* logits, const Rules a, int V, long ld, long ld_out, int chunks) {
+  constexpr int VEC = WIDE ? VocabRow<T>::VEC : 1, CHUNK = NT * U * VEC;
+  struct alignas(VEC * sizeof(T)) Word { T v[VEC]; };
+  __shared__ __attribute__((aligned(16))) uint32_t lds[CHUNK];
   const long row = blockIdx.x / chunks;
   const int part = blockIdx.x % chunks, tid = threadIdx.x;
-  const int slot = a.rows[row];
-  const bool ruled_row = slot >= 0 && slot < a.slots;
   const VocabRow<T> in(logits + row * ld, V);
   T* to = out + row * ld_out;
   // groups of VEC tokens; the first one of a row that starts inside a word is short
   const int lead = WIDE ? in.lead : 0, ahead = WIDE ? 1 : 0;
   const int all = ahead + (V - lead + VEC - 1) / VEC;
-  const int g0 = part * (chunk / VEC), g1 = min(g0 + chunk / VEC, all);
-  const int base = lead + (g0 - ahead) * VEC;     // token of LDS word 0, may be < 0
+  const int g0 = part * NT * U;
+  const int base = lead + (g0 - ahead) * VEC;     // the chunk's first token, may be < 0
+  // LDS word of the chunk's token t: a thread's VEC tokens in two halves (of 8), so that
+  // neighbours read neighbouring 16-byte words
+  auto at = [](int t) {
+    return VEC == 8 ? t / 8 * 4 + t % 4 + (t & 4) * (CHUNK / 8) : t;
+  };
   const bool same = out == logits;
+  Word v[U];
+  auto load = [&](int u) {
+    const int i0 = base + (u * NT + tid) * VEC;
+    if (i0 >= 0 && i0 + VEC <= V) {
+      v[u] = *reinterpret_cast<const Word*>(in.x + i0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (i0 + j >= 0 && i0 + j < V) v[u].v[j] = in.x[i0 + j];
+    }
+  };
+  const int slot = a.rows[row];
   float rep = 1.f, freq = 0.f, pres = 0.f;
   bool counts = false, biased = false, masked = false;
   int total = 0, prompt = 0;
-  if (ruled_row) {
+  if (slot >= 0 && slot < a.slots) {
     rep = a.repetition[slot], freq = a.frequency[slot], pres = a.presence[slot];
     total = min(max(a.total_len[slot], 0), a.cap);
     prompt = min(max(a.prompt_len[slot], 0), total);
@@ -80,71 +118,107 @@ __global__ __launch_bounds__(256) void logit_rules_kernel(
     masked = a.masked[slot] != 0;
   }
   if (same && !counts && !biased && !masked) return;
+  // What is read is on its way in the order in which it is needed, the logits last: they
+  // arrive while the history is counted.
+  const int* h = a.history + (long)slot * a.cap;
+  const int head = min((int)((16 - ((uintptr_t)h & 15)) & 15) / 4, total);
+  const int whole = counts ? (total - head) / 4 : 0, tail = head + whole * 4;
+  const i32x4_t* words = reinterpret_cast<const i32x4_t*>(h + head);
+  i32x4_t w[HW];
+  auto next_words = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < HW; ++k)
+      if (i + k * NT < whole) w[k] = words[i + k * NT];
+  };
+  next_words(tid);
+  int ends[2] = {-1, -1};               // tokens before and behind the words
+  if (counts && tid < head) ends[0] = h[tid];
+  if (counts && tid < total - tail) ends[1] = h[tail + tid];
+  const int* b = a.bias_tokens + (long)slot * a.biases;
+  const int bias0 = biased && tid < a.biases ? b[tid] : -1;
+  // in place only what is rewritten is read
+  if (!same || masked)
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(u);
+  uint32_t bits[U];
+  const int* mask = a.mask + (long)slot * a.words;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i0 = base + (u * NT + tid) * VEC;
+    bits[u] = ~0u;
+    const int lo = max(i0, 0), hi = min(i0 + VEC, V) - 1;
+    if (!masked || lo > hi) continue;
+    // bit j: token i0 + j is allowed
+    const uint64_t two = (uint32_t)mask[lo >> 5] |
+                         (uint64_t)(uint32_t)mask[hi >> 5] << 32;
+    bits[u] = (hi >> 5 == lo >> 5 ? (uint32_t)two >> (lo & 31)
+                                  : (uint32_t)(two >> (lo & 31))) << (lo - i0);
+  }
   const float* values = a.bias_values + (long)slot * a.biases;
   if (counts || biased) {
-    for (int i = tid; i < chunk; i += 256) lds[i] = 0;
-    __syncthreads();
+#pragma unroll
+    for (int i = tid * 4; i < CHUNK; i += NT * 4)
+      *reinterpret_cast<i32x4_t*>(lds + i) = i32x4_t{0, 0, 0, 0};
+    lds_barrier();
     if (counts) {
-      const int* h = a.history + (long)slot * a.cap;
-      for (int i = tid; i < total; i += 256) {
-        const int t = h[i] - base;
-        if ((unsigned)t < (unsigned)chunk && h[i] >= 0) {
-          if (i < prompt) atomicOr(&lds[t], SEEN);
-          else atomicAdd(&lds[t], 1u);
-        }
+      auto count = [&](int i, int token) {
+        const int t = token - base;
+        if ((unsigned)t >= (unsigned)CHUNK || token < 0) return;
+        if (i < prompt) atomicOr(&lds[at(t)], SEEN);
+        else atomicAdd(&lds[at(t)], 1u);
+      };
+      count(tid, ends[0]);
+      count(tail + tid, ends[1]);
+      for (int i = tid; i < whole; i += HW * NT) {
+        if (i != tid) next_words(i);
+#pragma unroll
+        for (int k = 0; k < HW; ++k)
+          if (i + k * NT < whole)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) count(head + (i + k * NT) * 4 + j, w[k][j]);
       }
-      __syncthreads();
+      lds_barrier();
     }
     // the last entry of a token holds; the lower bits stand still by now
     if (biased) {
-      const int* b = a.bias_tokens + (long)slot * a.biases;
-      for (int i = tid; i < a.biases; i += 256) {
-        const int t = b[i] - base;
-        if ((unsigned)t < (unsigned)chunk && b[i] >= 0)
-          atomicMax(&lds[t], (uint32_t)(i + 1) << BIAS |
-                                 (lds[t] & ((1u << BIAS) - 1)));
+      for (int i = tid; i < a.biases; i += NT) {
+        const int token = i == tid ? bias0 : b[i], t = token - base;
+        if ((unsigned)t < (unsigned)CHUNK && token >= 0)
+          atomicMax(&lds[at(t)], (uint32_t)(i + 1) << BIAS |
+                                     (lds[at(t)] & ((1u << BIAS) - 1)));
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
-  const int* mask = a.mask + (long)slot * a.words;
-  for (int g = g0 + tid; g < g1; g += 256) {
-    const int i0 = lead + (g - ahead) * VEC;
-    uint32_t w[VEC], any = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int t0 = (u * NT + tid) * VEC, i0 = base + t0;
+    if (i0 >= V) continue;
     if (counts || biased) {
+      uint32_t c[VEC], any = 0;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) any |= w[j] = lds[i0 - base + j];
-    }
-    if (same && !masked && any == 0) continue;
-    float v[VEC];
-    if (WIDE) {
-      float u[VocabRow<T>::VEC];
-      in.load(g, u);
+      for (int j = 0; j < VEC; ++j) any |= c[j] = lds[at(t0 + j)];
+      if (same && !masked) {
+        if (any == 0) continue;
+        load(u);
+      }
+      if (any != 0)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = u[j];
-    } else {
-      v[0] = (float)in.x[i0];
-    }
-    if (any != 0) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[j] = ruled(v[j], w[j], rep, freq, pres, values);
+        for (int j = 0; j < VEC; ++j)
+          if (c[j] != 0)
+            v[u].v[j] = rounded<T>(ruled((float)v[u].v[j], c[j], rep, freq, pres, values));
     }
     if (masked) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int i = i0 + j;
-        if (i >= 0 && i < V && !(mask[i >> 5] >> (i & 31) & 1)) v[j] = -INFINITY;
-      }
+      for (int j = 0; j < VEC; ++j)
+        if (!(bits[u] >> j & 1)) v[u].v[j] = rounded<T>(-INFINITY);
     }
-    if (WIDE && i0 >= 0 && i0 + VEC <= V) {
-      struct alignas(16) Vec { T v[VEC]; } o;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) o.v[j] = rounded<T>(v[j]);
-      *reinterpret_cast<Vec*>(to + i0) = o;
+    if (i0 >= 0 && i0 + VEC <= V) {
+      *reinterpret_cast<Word*>(to + i0) = v[u];
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        if (i0 + j >= 0 && i0 + j < V) to[i0 + j] = rounded<T>(v[j]);
+        if (i0 + j >= 0 && i0 + j < V) to[i0 + j] = v[u].v[j];
     }
   }
 }
@@ -215,21 +289,20 @@ void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
                 presence.data_ptr<float>(), bias_tokens.data_ptr<int>(),
                 bias_values.data_ptr<float>(), mask.data_ptr<int>(),
                 masked.data_ptr<int>(), (int)R, (int)cap, (int)nb, (int)mask.size(1)};
-  int chunk = 8192;
-  while (chunk > 1024 && N * ((V + chunk - 1) / chunk) < 512) chunk /= 2;
   auto go = [&](auto t) {
     using T = decltype(t);
-    const uintptr_t at = (uintptr_t)logits.data_ptr() ^ (uintptr_t)out.data_ptr();
-    const bool wide = (at & 15) == 0 &&
+    constexpr int VEC = 16 / sizeof(T);
+    const uintptr_t apart = (uintptr_t)logits.data_ptr() ^ (uintptr_t)out.data_ptr();
+    const bool wide = (apart & 15) == 0 &&
                       ((logits.stride(0) - out.stride(0)) * sizeof(T) & 15) == 0;
     // (a row that starts inside a word has one group more)
-    const long chunks = (V + (wide ? 16 / (long)sizeof(T) : 0) + chunk - 1) / chunk;
+    const int chunk = wide ? NT * VEC * 2 : NT * 16;
+    const long chunks = (V + (wide ? VEC : 0) + chunk - 1) / chunk;
     TORCH_CHECK(N * chunks < (1L << 31), "adjust_logits: too many rows");
-    auto kern = wide ? logit_rules_kernel<T, true> : logit_rules_kernel<T, false>;
-    kern<<<dim3((unsigned)(N * chunks)), dim3(256), chunk * 4,
-           at::hip::getCurrentHIPStream()>>>(
+    auto kern = wide ? logit_rules_kernel<T, true, 2> : logit_rules_kernel<T, false, 16>;
+    kern<<<dim3((unsigned)(N * chunks)), dim3(NT), 0, at::hip::getCurrentHIPStream()>>>(
         (T*)out.data_ptr(), (const T*)logits.data_ptr(), a, (int)V, logits.stride(0),
-        out.stride(0), chunk, (int)chunks);
+        out.stride(0), (int)chunks);
   };
   if (logits.scalar_type() == torch::kBFloat16) go(bf16_t{});
   else if (logits.scalar_type() == torch::kFloat32) go(float{});
