@@ -13,6 +13,7 @@ from . import ref
 
 MOST_ADAPTERS = 4095
 MOST_PARTS = 8
+MOST_RANK = 256
 
 
 class AdapterPlan:
@@ -56,8 +57,9 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
     (S, N, r): the S adapters of a projection of P parts whose ``widths`` add up to N
     (q, k and v of one fused product; default: one part).  scale (S,) fp32.  ranks (S,)
     int32: how much of r an adapter uses (0: none, its rows are y's); what a and b hold
-    beyond is not read.  ``out``: where the result goes, ``out=y`` in place.  bf16 or
-    fp32, all of one type."""
+    beyond is not read.  ``out``: where the result goes, ``out=y`` in place, else apart from
+    all operands.  bf16 or fp32, all of one type; at most 8 parts, r at most 256, K below
+    2^20.  The adapters a and b are contiguous, rows of y, x and out may lie apart."""
     widths = [y.shape[1]] if widths is None else [int(w) for w in widths]
     if torch.is_grad_enabled() and any(
             t.requires_grad for t in (y, x, a, b, scale)):
@@ -66,6 +68,13 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
     if plan.rows != y.shape[0]:
         raise ValueError(f"adapter_add: a plan of {plan.rows} rows for "
                          f"{y.shape[0]}")
+    if not 1 <= len(widths) <= MOST_PARTS or a.dim() != 4 \
+            or not 1 <= a.shape[2] <= MOST_RANK or a.shape[3] >= 1 << 20:
+        raise ValueError(f"adapter_add: 1 to {MOST_PARTS} parts, ranks 1 to "
+                         f"{MOST_RANK}, inner widths below 2^20")
+    if a.shape[0] != plan.slots:
+        raise ValueError(f"adapter_add: {a.shape[0]} adapters for a plan of "
+                         f"{plan.slots}")
     if y.is_cuda:
         from . import _NONE, _require_ext
         ext = _require_ext()

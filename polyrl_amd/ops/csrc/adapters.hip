@@ -10,7 +10,13 @@
 // one; all on the device, so that a captured decode step finds its tiles again.  ``down``
 // forms h = A x, the inner dimension cut over a block's waves and, where there are few
 // tiles, over blocks; ``up`` adds the blocks' shares in their order, multiplies with B
-// and adds the result to y, which it reads and writes once.
+// and adds the result to y, which it reads and writes once.  (One kernel for both would
+// read A in every block of columns; h is 1% of y.)
+//
+// What bounds it: memory, prompts by y and out (6504 rows, ranks 32, the four projections of
+// 4096 / 6144 / 14336 numbers, 1.43 GB: 404 us, 3.5 TB/s; the widest, 746 MB, 170 us, where a
+// copy of the same tiles takes 131), decode by the adapters (57 rows of as many adapters of
+// ranks 64 and 32, 0.45 GB: 152 us, 2.9 TB/s); one row by nine launches, 48 us.
 //
 // Matrix cores: 16x16x32 in bf16, 16x16x4 in fp32.  h is a sum in 32 bits; as an operand
 // in bf16 it is split in two bf16 numbers, h = hi + lo, each with its own product, so that what
@@ -49,14 +55,15 @@ template <> struct Operand<float> {
 };
 
 // p[0 .. have) of a lane's numbers, zeros behind.  WORDS: 16 bytes at p can be read
-// wherever have > 0
-template <typename T, bool WORDS>
+// wherever have > 0.  ONCE: nobody else reads them
+template <typename T, bool WORDS, bool ONCE = false>
 DEV_INLINE i32x4_t load_some(const T* p, int have) {
   constexpr int PER = Operand<T>::PER;
   if (have <= 0) return i32x4_t{0, 0, 0, 0};
   T v[PER];
   if (WORDS) {
-    const i32x4_t w = *reinterpret_cast<const i32x4_t*>(p);
+    const i32x4_t* at = reinterpret_cast<const i32x4_t*>(p);
+    const i32x4_t w = ONCE ? __builtin_nontemporal_load(at) : *at;
     if (have >= PER) return w;
     __builtin_memcpy(v, &w, 16);
   } else {
@@ -75,57 +82,79 @@ DEV_INLINE i32x4_t load_some(const T* p, int have) {
 // ---------------------------------------------------------------------- plan
 // plan: tiles, then (4 ints each) adapter, first place, rows; then the rows by place.
 // Rows without an adapter come last, as tiles of adapter -1.
+constexpr int XCDS = 8;               // dies, each with an L2 of its own
 constexpr int PLAN_HEAD = 4;
-constexpr int MOST_SLOTS = 4095;
+constexpr int MOST_SLOTS = 4095, MOST_RANK = 256;
+
+// the sum of the wave's lower lanes' numbers and this one's
+DEV_INLINE int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int below = __shfl_up(x, d, 64);
+    if (lane >= d) x += below;
+  }
+  return x;
+}
+
+// f(row, adapter, lanes): every row, with the lanes of the wave whose rows are of the same
+// adapter, as far as two rounds find them (a prompt's rows are all of one), else its own
+template <typename F>
+DEV_INLINE void by_adapter(const int* index, int T, int slots, F f) {
+  constexpr int U = 8;
+  for (int t0 = 0; t0 < T; t0 += U * 1024) {
+    int s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * 1024 + threadIdx.x;
+      s[u] = t < T ? index[t] : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * 1024 + threadIdx.x;
+      if (t0 + u * 1024 >= T) break;
+      if (s[u] < 0 || s[u] >= slots) s[u] = slots;
+      bool mine = t < T;
+      for (int r = 0; r < 2; ++r) {
+        const unsigned long long left = __ballot(mine);
+        if (left == 0) break;
+        const int first = __shfl(s[u], __ffsll(left) - 1, 64);
+        const bool now = mine && s[u] == first;
+        const unsigned long long same = __ballot(now);
+        if (now) f(t, s[u], same);
+        mine = mine && !now;
+      }
+      if (mine) f(t, s[u], 1ull << (threadIdx.x & 63));
+    }
+  }
+}
 
 __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int* index,
                                                             int T, int slots, int tile,
                                                             int most) {
   __shared__ int count[MOST_SLOTS + 1], cursor[MOST_SLOTS + 1];
-  __shared__ int sum_rows[1024], sum_tiles[1024];
-  const int tid = threadIdx.x;
+  __shared__ int sum_rows[16], sum_tiles[16];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   for (int s = tid; s <= slots; s += 1024) count[s] = 0;
   __syncthreads();
-  // rows of the wave's first row's adapter are counted by one lane, twice; a prompt's
-  // are all of them
-  for (int t0 = 0; t0 < T; t0 += 1024) {
-    const int t = t0 + tid;
-    int s = t < T ? index[t] : -2;
-    if (t < T && (s < 0 || s >= slots)) s = slots;
-    bool mine = s >= 0;
-    for (int r = 0; r < 2; ++r) {
-      const unsigned long long left = __ballot(mine);
-      if (left == 0) break;
-      const int first = __ffsll(left) - 1;
-      const int f = __shfl(s, first, 64);
-      const unsigned long long same = __ballot(mine && s == f);
-      if ((tid & 63) == first) atomicAdd(&count[f], __popcll(same));
-      if (s == f) mine = false;
-    }
-    if (mine) atomicAdd(&count[s], 1);
-  }
+  by_adapter(index, T, slots, [&](int, int s, unsigned long long lanes) {
+    if (__ffsll(lanes) - 1 == lane) atomicAdd(&count[s], __popcll(lanes));
+  });
   __syncthreads();
-  // each thread a stretch of adapters, then the stretches' sums
+  // each thread a stretch of adapters, then sums of the threads before
   const int per = (slots + 1 + 1023) / 1024;
   int rows = 0, tiles = 0;
   for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
     rows += count[s];
     tiles += (count[s] + tile - 1) / tile;
   }
-  sum_rows[tid] = rows;
-  sum_tiles[tid] = tiles;
+  int at = wave_scan(rows), n = wave_scan(tiles);
+  if (lane == 63) sum_rows[wid] = at, sum_tiles[wid] = n;
   __syncthreads();
-  for (int d = 1; d < 1024; d *= 2) {
-    const int r = tid >= d ? sum_rows[tid - d] : 0;
-    const int n = tid >= d ? sum_tiles[tid - d] : 0;
-    __syncthreads();
-    sum_rows[tid] += r;
-    sum_tiles[tid] += n;
-    __syncthreads();
-  }
-  if (tid == 1023) plan[0] = sum_tiles[1023];
+  for (int w = 0; w < wid; ++w) at += sum_rows[w], n += sum_tiles[w];
+  if (tid == 1023) plan[0] = n;
+  at -= rows, n -= tiles;
   i32x4_t* entry = reinterpret_cast<i32x4_t*>(plan + PLAN_HEAD);
-  int at = sum_rows[tid] - rows, n = sum_tiles[tid] - tiles;
   for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
     cursor[s] = at;
     for (int i = 0; i < count[s]; i += tile, ++n)
@@ -134,28 +163,13 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
   }
   __syncthreads();
   int* order = plan + PLAN_HEAD + 4 * most;
-  for (int t0 = 0; t0 < T; t0 += 1024) {
-    const int t = t0 + tid;
-    int s = t < T ? index[t] : -2;
-    if (t < T && (s < 0 || s >= slots)) s = slots;
-    bool mine = s >= 0;
-    for (int r = 0; r < 2; ++r) {
-      const unsigned long long left = __ballot(mine);
-      if (left == 0) break;
-      const int first = __ffsll(left) - 1;
-      const int f = __shfl(s, first, 64);
-      const bool now = mine && s == f;
-      const unsigned long long same = __ballot(now);
-      int place = 0;
-      if ((tid & 63) == first) place = atomicAdd(&cursor[f], __popcll(same));
-      place = __shfl(place, first, 64);
-      if (now) {
-        order[place + __popcll(same & ((1ull << (tid & 63)) - 1))] = t;
-        mine = false;
-      }
-    }
-    if (mine) order[atomicAdd(&cursor[s], 1)] = t;
-  }
+  by_adapter(index, T, slots, [&](int t, int s, unsigned long long lanes) {
+    const int first = __ffsll(lanes) - 1;
+    int place = 0;
+    if (first == lane) place = atomicAdd(&cursor[s], __popcll(lanes));
+    place = __builtin_amdgcn_ds_bpermute(first * 4, place);
+    order[place + __popcll(lanes & ((1ull << lane) - 1))] = t;
+  });
 }
 
 // ---------------------------------------------------------------------- down
@@ -166,62 +180,133 @@ struct Shape {
   int first[9];                       // columns of the parts
 };
 
-// h[share][place][part][j], one block a tile of rows, CT tiles of ranks of a part and a
-// share of the inner dimension
-template <typename T, int RT, int CT, bool WORDS>
-__global__ __launch_bounds__(256) void adapter_down_kernel(
+#ifndef MOST_REPS
+#define MOST_REPS 16
+#endif
+#ifndef UP_BLOCKS
+#define UP_BLOCKS 2048
+#endif
+constexpr int MOST_SPLIT = 4;
+
+// Operand tiles from rows that lie far apart.  The matrix cores want row l % 16 in lane l,
+// but the L1 takes a cycle for each lane of a load whose neighbours do not lie beside it
+// and 16 for four rows of 256 bytes (a kernel of loads alone, 6528 rows of 14336 bf16
+// numbers and 32 of A for every 32 of them: 57 us by lanes of 16 rows, 42 by 8 rows of 128
+// bytes, 41 by 4 of 256; this kernel 72 and 52).  So load j reads rows 4 * i + j, i = 0 .. 3,
+// a lane 16 bytes of row 4 * (l / 4 % 4) + j from 64 * (l / 16) + 16 * (l % 4), and every four
+// lanes transpose what they have: then load j's register holds row l % 16, bytes
+// 64 * (l / 16) + 16 * j.  (The order of the inner dimension is the same in both operands.)
+DEV_INLINE void quads_transposed(i32x4_t (&v)[4]) {
+  const bool one = threadIdx.x & 1, two = threadIdx.x & 2;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+#pragma unroll
+    for (int p = 0; p < 4; p += 2) {    // lane bit 0 and load bit 0
+      const int a = v[p][d], b = v[p + 1][d];
+      const int na = __builtin_amdgcn_mov_dpp(a, 0xb1, 0xf, 0xf, true);
+      const int nb = __builtin_amdgcn_mov_dpp(b, 0xb1, 0xf, 0xf, true);
+      v[p][d] = one ? nb : a;
+      v[p + 1][d] = one ? b : na;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {       // and 1
+      const int a = v[p][d], b = v[p + 2][d];
+      const int na = __builtin_amdgcn_mov_dpp(a, 0x4e, 0xf, 0xf, true);
+      const int nb = __builtin_amdgcn_mov_dpp(b, 0x4e, 0xf, 0xf, true);
+      v[p][d] = two ? nb : a;
+      v[p + 2][d] = two ? b : na;
+    }
+  }
+}
+
+// h[share][place][part][j].  A block takes RT * 16 rows of a tile, CT tiles of 16 ranks
+// (tile i: ranks 16 * (i / parts) .. of part i % parts) and a share of the inner
+// dimension, each of its NW waves a part of that
+template <typename T, int NW, int RT, int CT, bool WORDS>
+__global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
     float* __restrict__ h, const T* __restrict__ x, const T* __restrict__ a,
-    const int* __restrict__ ranks, const int* __restrict__ plan, const Shape z) {
+    const int* __restrict__ ranks, const int* __restrict__ plan, const Shape z,
+    int subs) {
   using O = Operand<T>;
-  __shared__ float red[4 * RT * CT * 256];
+  __shared__ float red[NW * RT * CT * 256];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
-  const int groups = (z.rank16 / 16 + CT - 1) / CT;
-  int id = blockIdx.x;
+  const int groups = (z.rank16 / 16 * z.parts + CT - 1) / CT;
+  // A die takes a stretch of the tiles, which lie in the order of their adapters: few
+  // adapters' matrices for each L2.  Reads wait for each other in three steps: the tile;
+  // its rows and the adapter's rank; what they name.
+  const int n = plan[0] * subs, stretch = (n + XCDS - 1) / XCDS;
+  int id = blockIdx.x / XCDS;
   const int share = id % z.split;
   id /= z.split;
   const int group = id % groups;
   id /= groups;
-  const int part = id % z.parts, tile = id / z.parts;
-  if (tile >= plan[0]) return;
+  const int at = blockIdx.x % XCDS * stretch + id;
+  if (id >= stretch || at >= n) return;
+  const int tile = at / subs, sub = at % subs;
   const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[tile];
-  const int slot = t[0], place = t[1], rows = t[2];
-  if (slot < 0) return;
+  const int slot = t[0], place = t[1] + sub * RT * 16, rows = t[2] - sub * RT * 16;
+  if (slot < 0 || rows <= 0) return;
   const int rank = ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
-  const int j0 = group * CT * 16;
-  if (j0 >= rank) return;
   const int* order = plan + PLAN_HEAD + 4 * z.most + place;
-  // this wave's share of the inner dimension, in whole lines of 128 bytes
-  const int line = 128 / (int)sizeof(T), lines = (z.K + line - 1) / line;
-  const int per = (lines + z.split * 4 - 1) / (z.split * 4) * line;
-  const int k0 = (share * 4 + wid) * per, k1 = min(k0 + per, z.K);
-  const T* xr[RT];
-  const T* ar[CT];
+  // rows of load j, and where this lane starts in them; rows past the tile and ranks
+  // past the adapter's are any, dropped below
+  const int first = lane / 4 % 4 * 4, part_of = (lhi * 4 + lane % 4) * O::PER;
+  const T* xr[RT][4];
+  const T* base[CT];
+  uint32_t ar[CT][4];                 // (a matrix is less than 2^30 bytes)
 #pragma unroll
-  for (int r = 0; r < RT; ++r)        // rows past the tile: any, dropped below
-    xr[r] = x + (long)order[min(r * 16 + l15, rows - 1)] * z.ldx + lhi * O::PER;
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
-    ar[c] = a + (((long)slot * z.parts + part) * z.rank +
-                 min(j0 + c * 16 + l15, rank - 1)) * z.K + lhi * O::PER;
+    for (int j = 0; j < 4; ++j)
+      xr[r][j] = x + (long)order[min(r * 16 + first + j, rows - 1)] * z.ldx + part_of;
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int i = group * CT + c;
+    base[c] = a + ((long)slot * z.parts + i % z.parts) * z.rank * z.K;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ar[c][j] = (uint32_t)min(i / z.parts * 16 + first + j, z.rank - 1) * (uint32_t)z.K +
+                 (uint32_t)part_of;
+  }
+  if (group * CT / z.parts * 16 >= rank) return;
   f32x4_t acc[RT][CT];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[r][c] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = k0; k < k1; k += O::STEP) {
-    const int have = k1 - k - lhi * O::PER;
-    i32x4_t xv[RT], av[CT];
+  // this wave's part of the inner dimension, 256 bytes a round
+  constexpr int ROUND = 4 * O::STEP;
+  const int rounds = (z.K + ROUND - 1) / ROUND;
+  const int per = (rounds + z.split * NW - 1) / (z.split * NW) * ROUND;
+  const int k0 = (share * NW + wid) * per, k1 = min(k0 + per, z.K);
+  auto round = [&](int k, auto whole) {
+    i32x4_t xv[RT][4], av[CT][4];
+    const int have = decltype(whole)::value ? O::PER : k1 - k - part_of;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) xv[r] = load_some<T, WORDS>(xr[r] + k, have);
+    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) av[c] = load_some<T, WORDS>(ar[c] + k, have);
+      for (int c = 0; c < CT; ++c)
+        av[c][j] = load_some<T, WORDS>(base[c] + k + ar[c][j], have);
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+      for (int r = 0; r < RT; ++r) xv[r][j] = load_some<T, WORDS>(xr[r][j] + k, have);
+    }
 #pragma unroll
-      for (int c = 0; c < CT; ++c) acc[r][c] = O::mul(xv[r], av[c], acc[r][c]);
-  }
-  // sums of the four waves; register i: row 4 * (lane / 16) + i, column lane % 16
+    for (int c = 0; c < CT; ++c) quads_transposed(av[c]);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      quads_transposed(xv[r]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[r][c] = O::mul(xv[r][j], av[c][j], acc[r][c]);
+    }
+  };
+  int k = k0;
+#pragma unroll 1
+  for (; k + ROUND <= k1; k += ROUND) round(k, std::true_type());
+  if (k < k1) round(k, std::false_type());
+  // sums of the waves; register i: row 4 * (lane / 16) + i, column lane % 16
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -230,125 +315,283 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(
       for (int i = 0; i < 4; ++i)
         red[((wid * RT + r) * CT + c) * 256 + (lhi * 4 + i) * 16 + l15] = acc[r][c][i];
   __syncthreads();
-  const int row = threadIdx.x / 16, col = threadIdx.x % 16;
+  for (int o = threadIdx.x; o < RT * CT * 256; o += NW * 64) {
+    const int i = group * CT + o / 256 % CT, r = o / 256 / CT;
+    const int row = r * 16 + o % 256 / 16, j = i / z.parts * 16 + o % 16;
+    if (row >= rows || j >= rank) continue;
+    float v = 0.f;
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-        v += red[((w * RT + r) * CT + c) * 256 + threadIdx.x];
-      const int j = j0 + c * 16 + col;
-      if (r * 16 + row < rows && j < rank)
-        h[(((long)share * z.T + place + r * 16 + row) * z.parts + part) * z.rank16 + j] = v;
-    }
+    for (int w = 0; w < NW; ++w) v += red[w * RT * CT * 256 + o];
+    h[(((long)share * z.T + place + row) * z.parts + i % z.parts) * z.rank16 + j] = v;
+  }
 }
 
 // ------------------------------------------------------------------------ up
-// A block takes a tile of rows and 256 columns of one part, a wave 64 of them as four
-// tiles of 16, which are dealt so that a lane holds 16 neighbouring columns of its row:
-// tile c's row i is column 16 * (i / 4) + 4 * c + i % 4.
-constexpr int UP_COLS = 256, UP_RANK = 64;
+// h's numbers j .. j + 4 of a place, times s: the shares' sums in their order, split into hi
+// and lo; zeros from rank on
+template <typename T>
+struct Four {
+  T hi[4], lo[4];
+  DEV_INLINE Four(f32x4_t v, float s, int left) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = e < left ? v[e] * s : 0.f;
+      hi[e] = (T)f;
+      // (an infinite h has no lower part)
+      lo[e] = isfinite((float)hi[e]) ? (T)(f - (float)hi[e]) : (T)0.f;
+    }
+  }
+  DEV_INLINE static void put(T* at, const T (&v)[4]) {
+    struct alignas(sizeof(T) * 4) Word { T v[4]; };
+    Word w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w.v[e] = v[e];
+    *reinterpret_cast<Word*>(at) = w;
+  }
+};
+DEV_INLINE f32x4_t shares_sum(const float* p, long share, int split) {
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < MOST_SPLIT; ++w)
+    if (w < split) v += *reinterpret_cast<const f32x4_t*>(p + w * share);
+  return v;
+}
 
+// Where a block of ``wide`` columns stands: a tile, a part and its columns n0 .. end
+struct Place {
+  int tile, part, n0, end;
+  DEV_INLINE Place(const Shape& z, int cols, int wide) : tile(blockIdx.x / cols), part(0) {
+    int col = blockIdx.x % cols;
+    while (col >= (z.first[part + 1] - z.first[part] + wide - 1) / wide) {
+      col -= (z.first[part + 1] - z.first[part] + wide - 1) / wide;
+      ++part;
+    }
+    n0 = z.first[part] + col * wide, end = z.first[part + 1];
+  }
+};
+
+// Few rows: a tile of 16, where b is most of what is read.  A wave takes 64 columns, b
+// straight into its operands, as four tiles whose columns are dealt so that a lane holds
+// whole 16-byte words of its row l % 16: word q is columns 4 * VEC * q + VEC * (l / 16) ..
 // WORDS: rows of b come in whole 16-byte words; OUT_WORDS: those of y and out
-template <typename T, int RT, bool WORDS, bool OUT_WORDS>
-__global__ __launch_bounds__(256) void adapter_up_kernel(
+constexpr int FEW_COLS = 256, FEW_RANK = 64;
+
+template <typename T, bool WORDS, bool OUT_WORDS>
+__global__ __launch_bounds__(256) void adapter_up_few_kernel(
     T* out, const T* y, const float* __restrict__ h, const T* __restrict__ b,
     const float* __restrict__ scale, const int* __restrict__ ranks,
     const int* __restrict__ plan, const Shape z, int cols) {
   using O = Operand<T>;
   constexpr bool SPLIT = sizeof(T) == 2;          // h as hi + lo
-  constexpr int PITCH = UP_RANK + 16 / (int)sizeof(T);
-  __shared__ __attribute__((aligned(16))) T hs[SPLIT ? 2 : 1][RT * 16][PITCH];
+  constexpr int VEC = 16 / (int)sizeof(T), Q = 16 / VEC, PER_Q = VEC / 4;
+  constexpr int PITCH = FEW_RANK + VEC, S = FEW_RANK / O::STEP;
+  struct alignas(16) Word { T v[VEC]; };
+  __shared__ __attribute__((aligned(16))) T hs[SPLIT ? 2 : 1][16][PITCH];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
-  const int tile = blockIdx.x / cols;
-  int col = blockIdx.x % cols, part = 0;
-  if (tile >= plan[0]) return;
-  while (col >= (z.first[part + 1] - z.first[part] + UP_COLS - 1) / UP_COLS) {
-    col -= (z.first[part + 1] - z.first[part] + UP_COLS - 1) / UP_COLS;
-    ++part;
-  }
-  const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[tile];
+  const Place at(z, cols, FEW_COLS);
+  if (at.tile >= plan[0]) return;
+  const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[at.tile];
   const int slot = t[0], place = t[1], rows = t[2];
+  if (slot < 0 && out == y) return;
   const int rank = slot < 0 ? 0 : ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
-  if (rank == 0 && out == y) return;
-  const int* order = plan + PLAN_HEAD + 4 * z.most + place;
-  const int end = z.first[part + 1];
-  const int n0 = z.first[part] + col * UP_COLS + wid * 64;
-  const float s = slot < 0 ? 0.f : scale[slot];
-  f32x4_t acc[RT][4];
+  const int n0 = at.n0 + wid * 64, end = at.end;
+  const bool whole = OUT_WORDS && n0 + 64 <= end;
+  // all that is read is on its way before any of it is waited for
+  const long row = (plan + PLAN_HEAD + 4 * z.most + place)[min(l15, rows - 1)];
+  const T* bb = b + (long)max(slot, 0) * z.N * z.rank;
+  i32x4_t bv[S][4];
+  auto load_b = [&](int j0) {
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+    for (int k = 0; k < S; ++k)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[r][c] = {0.f, 0.f, 0.f, 0.f};
-  const T* br[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c)                     // columns past the part: its last
-    br[c] = b + ((long)max(slot, 0) * z.N +
-                 min(n0 + l15 / 4 * 16 + c * 4 + l15 % 4, end - 1)) * z.rank +
-            lhi * O::PER;
-  for (int j0 = 0; j0 < rank; j0 += UP_RANK) {
-    const int have = min(rank - j0, UP_RANK);
-    if (j0 > 0) __syncthreads();
-    for (int i = threadIdx.x; i < RT * 16 * UP_RANK; i += 256) {
-      const int r = i / UP_RANK, j = i % UP_RANK;
-      float v = 0.f;
-      if (r < rows && j < have) {
-        const float* p = h + (((long)place + r) * z.parts + part) * z.rank16 + j0 + j;
-        for (int w = 0; w < z.split; ++w)
-          v += p[(long)w * z.T * z.parts * z.rank16];
-        v *= s;
+      for (int c = 0; c < 4; ++c) {               // columns past the part: its last
+        const int n = n0 + c / PER_Q * 4 * VEC + l15 / 4 * VEC + c % PER_Q * 4 + l15 % 4;
+        const int j = j0 + k * O::STEP + lhi * O::PER;
+        bv[k][c] = load_some<T, WORDS>(bb + (long)min(n, end - 1) * z.rank + j, rank - j);
       }
-      const T hi = (T)v;
-      hs[0][r][j] = hi;
-      // (an infinite h has no lower part)
-      if (SPLIT) hs[SPLIT ? 1 : 0][r][j] = isfinite((float)hi) ? (T)(v - (float)hi) : (T)0.f;
+  };
+  load_b(0);
+  Word yv[Q];
+  if (whole)
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      yv[q] = *reinterpret_cast<const Word*>(y + row * z.ldy + n0 + q * 4 * VEC + lhi * VEC);
+  const float s = slot < 0 ? 0.f : scale[slot];
+  f32x4_t acc[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int j0 = 0; j0 < rank; j0 += FEW_RANK) {
+    if (j0 > 0) {
+      load_b(j0);
+      __syncthreads();
+    }
+    const int r = threadIdx.x / 16, j = threadIdx.x % 16 * 4;
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (r < rows && j0 + j < rank)
+      v = shares_sum(h + (((long)place + r) * z.parts + at.part) * z.rank16 + j0 + j,
+                     (long)z.T * z.parts * z.rank16, z.split);
+    const Four<T> f(v, s, rank - j0 - j);
+    f.put(&hs[0][r][j], f.hi);
+    if (SPLIT) f.put(&hs[SPLIT ? 1 : 0][r][j], f.lo);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < S; ++k) {
+      if (j0 + k * O::STEP >= rank) break;
+#pragma unroll
+      for (int p = 0; p < (SPLIT ? 2 : 1); ++p) {
+        const i32x4_t hv =
+            *reinterpret_cast<const i32x4_t*>(&hs[p][l15][k * O::STEP + lhi * O::PER]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] = O::mul(bv[k][c], hv, acc[c]);
+      }
+    }
+  }
+  if (l15 >= rows || (rank == 0 && out == y)) return;
+  // register i of tile c: row lane % 16, column 4 * (lane / 16) + i of the tile's
+  if (whole) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      Word w = yv[q];
+      if (rank > 0)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          w.v[e] = (T)((float)w.v[e] + acc[q * PER_Q + e / 4][e % 4]);
+      *reinterpret_cast<Word*>(out + row * z.ldo + n0 + q * 4 * VEC + lhi * VEC) = w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int n = n0 + i / VEC * 4 * VEC + lhi * VEC + i % VEC;
+      if (n >= end) continue;
+      const T old = y[row * z.ldy + n];
+      out[row * z.ldo + n] = rank > 0 ? (T)((float)old + acc[i / 4][i % 4]) : old;
+    }
+  }
+}
+
+// Many rows, where y and out are most of it: a block takes a tile of 64, 16 for each wave,
+// and 16 * VEC columns as VEC tiles, which are dealt so that a lane has VEC neighbouring
+// columns of a row, a 16-byte word, and 16 lanes 256 bytes of it: tile c's column i is
+// VEC * i + c.  b and h go through LDS, PRE ranks at a time, b's rows in the tiles' order.
+// (6504 rows of 28672 columns, rank 32: lanes by rows as above for few 220 us, so 185, with
+// registers for four blocks a CU 170; for five they spill, 363.  A wave that keeps its
+// columns of b and goes through the rows, their loads a round ahead, has too few of
+// them on their way: 243 to 345.)
+template <typename T, int PRE, bool WORDS, bool OUT_WORDS>
+__global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
+    T* out, const T* y, const float* __restrict__ h, const T* __restrict__ b,
+    const float* __restrict__ scale, const int* __restrict__ ranks,
+    const int* __restrict__ plan, const Shape z, int cols) {
+  using O = Operand<T>;
+  constexpr bool SPLIT = sizeof(T) == 2;          // h as hi + lo
+  constexpr int VEC = 16 / (int)sizeof(T), COLS = 16 * VEC, PITCH = PRE + VEC;
+  constexpr int GRAN = PRE / VEC;                 // 16-byte words of a row in LDS
+  struct alignas(16) Word { T v[VEC]; };
+  __shared__ __attribute__((aligned(16))) T bs[COLS][PITCH], hs[SPLIT ? 2 : 1][64][PITCH];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int l15 = lane & 15, lhi = lane >> 4;
+  const Place at(z, cols, COLS);
+  if (at.tile >= plan[0]) return;
+  const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[at.tile];
+  const int slot = t[0], place = t[1], rows = t[2];
+  if (slot < 0 && out == y) return;
+  const int rank = slot < 0 ? 0 : ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
+  const int* order = plan + PLAN_HEAD + 4 * z.most + place;
+  const int n0 = at.n0, end = at.end;
+  const float s = slot < 0 ? 0.f : scale[slot];
+  const int mine = wid * 16 + lhi * 4;            // this lane's first row
+  const bool whole = OUT_WORDS && n0 + COLS <= end;
+  long row[4];
+  Word yv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = order[min(mine + i, rows - 1)];
+  constexpr int NB = COLS * GRAN / (256);     // words of b that a thread brings
+  constexpr int NH = 64 * PRE / 4 / (256);
+  const long share = (long)z.T * z.parts * z.rank16;
+  const T* bb = b + ((long)max(slot, 0) * z.N + n0) * z.rank;
+  const float* hh = h + ((long)place * z.parts + at.part) * z.rank16;
+  i32x4_t bv[NB];
+  f32x4_t hv[NH];
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {                // columns past the part: its last
+      const int g = threadIdx.x + i * 256, n = g / GRAN, j = j0 + g % GRAN * VEC;
+      bv[i] = load_some<T, WORDS>(bb + (uint32_t)(min(n, end - n0 - 1) * z.rank + j),
+                                  rank - j);
+    }
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      const int g = threadIdx.x + i * 256, r = g / (PRE / 4), j = j0 + g % (PRE / 4) * 4;
+      hv[i] = {0.f, 0.f, 0.f, 0.f};
+      if (r >= rows || j >= rank) continue;
+      hv[i] = shares_sum(hh + (uint32_t)(r * z.parts * z.rank16 + j), share, z.split);
+    }
+  };
+  fetch(0);
+  if (whole)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      yv[i] = *reinterpret_cast<const Word*>(y + row[i] * z.ldy + n0 + l15 * VEC);
+  if (rank == 0 && out == y) return;
+  f32x4_t acc[VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) acc[c] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int j0 = 0; j0 < rank; j0 += PRE) {
+    if (j0 > 0) {
+      fetch(j0);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int g = threadIdx.x + i * 256, n = g / GRAN;
+      *reinterpret_cast<i32x4_t*>(&bs[n % VEC * 16 + n / VEC][g % GRAN * VEC]) = bv[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      const int g = threadIdx.x + i * 256, r = g / (PRE / 4), j = g % (PRE / 4) * 4;
+      const Four<T> f(hv[i], s, rank - j0 - j);
+      f.put(&hs[0][r][j], f.hi);
+      if (SPLIT) f.put(&hs[SPLIT ? 1 : 0][r][j], f.lo);
     }
     __syncthreads();
-    for (int k = 0; k < have; k += O::STEP) {
-      i32x4_t bv[4];
+    if (wid * 16 < rows)
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        bv[c] = load_some<T, WORDS>(br[c] + j0 + k, have - k - lhi * O::PER);
+      for (int k = 0; k < PRE; k += O::STEP) {
+        if (j0 + k >= rank) break;
+        i32x4_t hw[SPLIT ? 2 : 1];
 #pragma unroll
-      for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
+        for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
+          hw[p] = *reinterpret_cast<const i32x4_t*>(&hs[p][wid * 16 + l15][k + lhi * O::PER]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const i32x4_t hv = *reinterpret_cast<const i32x4_t*>(
-              &hs[p][r * 16 + l15][k + lhi * O::PER]);
+        for (int c = 0; c < VEC; ++c) {
+          const i32x4_t bw =
+              *reinterpret_cast<const i32x4_t*>(&bs[c * 16 + l15][k + lhi * O::PER]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[r][c] = O::mul(bv[c], hv, acc[r][c]);
+          for (int p = 0; p < (SPLIT ? 2 : 1); ++p) acc[c] = O::mul(hw[p], bw, acc[c]);
         }
-    }
-  }
-  // lane: row lane % 16 of every 16, columns 16 * (lane / 16) .. + 16
-  const int n = n0 + lhi * 16;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if (r * 16 + l15 >= rows) continue;
-    const long row = order[r * 16 + l15];
-    const T* from = y + row * z.ldy + n;
-    T* to = out + row * z.ldo + n;
-    struct alignas(16) Word { T v[16 / sizeof(T)]; };
-    constexpr int VEC = 16 / (int)sizeof(T);
-    if (OUT_WORDS && n + 16 <= end) {
-#pragma unroll
-      for (int q = 0; q < 16 / VEC; ++q) {
-        Word w = reinterpret_cast<const Word*>(from)[q];
-        if (rank > 0) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i)
-            w.v[i] = (T)((float)w.v[i] + acc[r][(q * VEC + i) / 4][(q * VEC + i) % 4]);
-        }
-        reinterpret_cast<Word*>(to)[q] = w;
       }
+  }
+  // register i of tile c: row 4 * (lane / 16) + i, column VEC * (lane % 16) + c
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (mine + i >= rows) break;
+    if (whole) {
+      Word w = yv[i];
+      if (rank > 0)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) w.v[c] = (T)((float)w.v[c] + acc[c][i]);
+      *reinterpret_cast<Word*>(out + row[i] * z.ldo + n0 + l15 * VEC) = w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n + i < end)
-          to[i] = rank > 0 ? (T)((float)from[i] + acc[r][i / 4][i % 4]) : from[i];
+      for (int c = 0; c < VEC; ++c) {
+        const int n = n0 + l15 * VEC + c;
+        if (n >= end) break;
+        const T old = y[row[i] * z.ldy + n];
+        out[row[i] * z.ldo + n] = rank > 0 ? (T)((float)old + acc[c][i]) : old;
+      }
     }
   }
 }
@@ -385,39 +628,60 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
                                bool words_down, bool words_up, bool words_out) {
   auto stream = at::hip::getCurrentHIPStream();
   const int* pl = plan.data_ptr<int>();
-  const int RT = tile_rows(z.T) / 16, tiles16 = z.rank16 / 16;
-  const int CT = tiles16 >= 3 ? 4 : tiles16;
-  const int groups = (tiles16 + CT - 1) / CT;
-  const long blocks = (long)z.most * z.parts * groups;
-  z.split = (int)std::max<long>(1, std::min<long>({768 / blocks, z.K / 256, 16}));
+  // Tiles of ranks that a block takes: all of them in equal groups of up to three or four
+  // Up to 1024 rows a block takes 16 of them in 16 waves, else 32 in 8: of few rows there
+  // are too few blocks otherwise, of many each one reads A again (620 rows, fp32, 8960 -> 20
+  // 21 us in blocks of 32 rows and 16 of 16; 6504 rows, bf16, 14336 -> 32, before the
+  // loads were dealt as they are, 72 and 97).
+  const int sixteens = tile_rows(z.T) / 16, RT = z.T <= 1024 ? 1 : 2, NW = 16 / RT;
+  const int subs = sixteens / RT;
+  // Tiles of ranks that a block takes: all of them in equal groups, of up to two where a wave
+  // of 16 has 128 registers (three spill: 128 rows, 3 x 16 ranks of 4096, 8.0 us and 6.5 by
+  // two; 57 rows, 3 x 64 ranks of 3584 16.2 and 19.2, 2 x 64 15.0 and 11.8), of up to four
+  // where it has twice as many and reads x for each group
+  const int tiles = z.rank16 / 16 * z.parts, most_ct = RT == 1 ? 2 : 4;
+  const int groups = (tiles + most_ct - 1) / most_ct, CT = (tiles + groups - 1) / groups;
+  const long blocks = ((long)z.most * subs + XCDS - 1) / XCDS * XCDS *
+                      ((tiles + CT - 1) / CT);
+  // shares of the inner dimension until there are 512 blocks, each wave with a round at
+  // least; no more than up to four, because up adds them in every block
+  z.split = (int)std::max<long>(
+      1, std::min<long>({512 / blocks, (long)z.K * y.element_size() / (NW * 256),
+                         MOST_SPLIT}));
   auto h = torch::empty({(long)z.split * z.T * z.parts * z.rank16},
                         y.options().dtype(torch::kFloat32));
   TORCH_CHECK(blocks * z.split < (1L << 31), "adapter_add: too many rows");
-  auto down = [&](auto kern) {
-    kern<<<dim3((unsigned)(blocks * z.split)), dim3(256), 0, stream>>>(
-        h.data_ptr<float>(), (const T*)x.data_ptr(), (const T*)a.data_ptr(), ranks, pl, z);
+  auto down = [&](auto kern, int waves) {
+    kern<<<dim3((unsigned)(blocks * z.split)), dim3(waves * 64), 0, stream>>>(
+        h.data_ptr<float>(), (const T*)x.data_ptr(), (const T*)a.data_ptr(), ranks, pl, z,
+        subs);
   };
-#define DOWN(R, C)                                          \
-  if (RT == R && CT == C) {                                 \
-    words_down ? down(adapter_down_kernel<T, R, C, true>)   \
-               : down(adapter_down_kernel<T, R, C, false>); \
-  }
-  DOWN(1, 1) DOWN(1, 2) DOWN(1, 4) DOWN(4, 1) DOWN(4, 2) DOWN(4, 4)
+#define DOWN(N, R, C, W)                                         \
+  if (RT == R && CT == C && words_down == W)                     \
+    down(adapter_down_kernel<T, N, R, C, W>, N);
+#define DOWNS(N, R, C) DOWN(N, R, C, true) DOWN(N, R, C, false)
+  DOWNS(16, 1, 1) DOWNS(16, 1, 2)
+  DOWNS(8, 2, 1) DOWNS(8, 2, 2) DOWNS(8, 2, 3) DOWNS(8, 2, 4)
+#undef DOWNS
 #undef DOWN
   HIP_CHECK_KERNEL();
+  const int wide = sixteens == 1 ? FEW_COLS : 16 * 16 / (int)sizeof(T);
   int cols = 0;
   for (int p = 0; p < z.parts; ++p)
-    cols += (z.first[p + 1] - z.first[p] + UP_COLS - 1) / UP_COLS;
+    cols += (z.first[p + 1] - z.first[p] + wide - 1) / wide;
   TORCH_CHECK((long)z.most * cols < (1L << 31), "adapter_add: too many rows");
   auto up = [&](auto kern) {
     kern<<<dim3((unsigned)((long)z.most * cols)), dim3(256), 0, stream>>>(
         (T*)out.data_ptr(), (const T*)y.data_ptr(), h.data_ptr<float>(),
         (const T*)b.data_ptr(), scale.data_ptr<float>(), ranks, pl, z, cols);
   };
-#define UP(R, W, O) \
-  if (RT == R && words_up == W && words_out == O) up(adapter_up_kernel<T, R, W, O>);
-  UP(1, true, true) UP(1, true, false) UP(1, false, true) UP(1, false, false)
-  UP(4, true, true) UP(4, true, false) UP(4, false, true) UP(4, false, false)
+#define UP(W, O)                                                        \
+  if (words_up == W && words_out == O) {                                \
+    if (sixteens == 1) up(adapter_up_few_kernel<T, W, O>);              \
+    else if (z.rank <= 32) up(adapter_up_kernel<T, 32, W, O>);          \
+    else up(adapter_up_kernel<T, 64, W, O>);                            \
+  }
+  UP(true, true) UP(true, false) UP(false, true) UP(false, false)
 #undef UP
   HIP_CHECK_KERNEL();
 }
@@ -432,9 +696,9 @@ void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Ten
   TORCH_CHECK(x.size(0) == T && a.size(3) == K && a.size(1) == (long)widths.size() &&
                   b.size(0) == S && b.size(1) == N && b.size(2) == r && S == slots,
               "adapter_add: shapes that do not fit together");
-  TORCH_CHECK(widths.size() >= 1 && widths.size() <= 8 && r >= 1 && r <= 4096 &&
-                  K >= 1 && K < (1L << 30) && N < (1L << 30),
-              "adapter_add: 1 to 8 parts, ranks 1 to 4096");
+  TORCH_CHECK(widths.size() >= 1 && widths.size() <= 8 && r >= 1 && r <= MOST_RANK &&
+                  K >= 1 && K < (1L << 20) && N < (1L << 30),
+              "adapter_add: 1 to 8 parts, ranks 1 to ", MOST_RANK, ", inner widths below 2^20");
   for (const auto& t : {out, x, a, b})
     TORCH_CHECK(t.device() == y.device() && t.scalar_type() == y.scalar_type(),
                 "adapter_add: tensors of one type and device");

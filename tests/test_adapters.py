@@ -67,6 +67,14 @@ SIZES = [
     (300, 520, (130,), 100, 7),
     (64, 4096, (32,), 16, 2),
     (3, 1, (1,), 1, 1),
+    # both sides of the rows from which blocks are larger, ranks that need more than one
+    # round, several parts whose ranks fall into several groups
+    (1024, 136, (130, 30), 48, 2),
+    (1025, 136, (130, 30), 48, 2),
+    (1100, 4096, (256, 64, 64), 96, 2),
+    (40, 2050, (20, 20, 20), 130, 3),
+    (130, 600, (8, 8, 8, 8, 8, 8, 8, 8), 256, 2),
+    (258, 300, (70, 0, 5), 256, 4),
 ]
 
 
@@ -255,6 +263,15 @@ def test_refusals(dev):
         ops.adapter_add(y, x, a, b[:, :15], scale, plan)
     with pytest.raises(error):
         ops.adapter_add(y, x, a.clone().requires_grad_(), b, scale, plan)
+    with pytest.raises(error):                              # ranks beyond 256
+        ops.adapter_add(y, x, a.new_zeros(2, 1, 257, 32), b.new_zeros(2, 16, 257),
+                        scale, plan)
+    with pytest.raises(error):                              # nine parts
+        ops.adapter_add(y, x, a.new_zeros(2, 9, 8, 32), b, scale, plan,
+                        [8] + [1] * 8)
+    with pytest.raises(error):                              # other adapters
+        ops.adapter_add(y, x, a[:1].contiguous(), b[:1].contiguous(), scale[:1],
+                        plan)
     if dev == "cuda":
         for bad in (x.float(), x.half()):
             with pytest.raises(error):
@@ -265,6 +282,5 @@ def test_refusals(dev):
             ops.adapter_add(y, x, a, b, scale.double(), plan)
         with pytest.raises(error):
             ops.adapter_add(y, x, a.cpu(), b, scale, plan)
-        with pytest.raises(error):                          # a plan of other adapters
-            ops.adapter_add(y, x, a[:1].contiguous(), b[:1].contiguous(), scale[:1],
-                            plan)
+        with pytest.raises(error):
+            ops.adapter_add(y, x, a.transpose(2, 3), b, scale, plan)
