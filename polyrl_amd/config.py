@@ -29,6 +29,8 @@ class ModelConfig:
     use_remove_padding: bool = True
     lora_rank: int = 0
     lora_alpha: float = 16.0
+    # dropout of the adapters' inputs while training (seeded, no mask kept)
+    lora_dropout: float = 0.0
     trust_remote_code: bool = False
 
 

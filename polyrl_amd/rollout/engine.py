@@ -17,15 +17,17 @@ from __future__ import annotations
 import math
 import time
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional
+from typing import Callable, Dict, List, Optional
 
 import numpy as np
 import torch
 
 import polyrl_amd.ops as ops
 from ..models.registry import DecoderConfig
+from .adapters import AdapterPool
 from .kv_cache import (PagedKVCache, PagedLatentCache, RadixCache,
                        StateSlots)
+from .rules import RequestRules
 
 
 def _mm_nt(x: torch.Tensor, w: torch.Tensor, search: bool = True
@@ -109,6 +111,26 @@ class SamplingParams:
     top_p: float = 1.0
     max_new_tokens: int = 128
     stop_token_ids: tuple = ()
+    # rules on the next token (ops.adjust_logits); logprobs stay those of the
+    # model's own distribution.  Penalties: > 1 (repetition) and > 0 make tokens
+    # of prompt and output (repetition) or of the output less likely
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: tuple = ()        # (token, value) pairs or a dict; -inf bans
+    allowed_token_ids: tuple = ()   # empty: all
+    # grammars: f(output ids) -> the token ids that may come next, or int32
+    # words of them (ops.token_words), None for all; no token ends the request
+    token_mask: Optional[Callable] = None
+    # name of a loaded adapter (Engine.load_adapter), empty: the base model
+    adapter: str = ""
+
+    @property
+    def has_rules(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0
+                or self.presence_penalty != 0.0 or len(self.logit_bias) > 0
+                or len(self.allowed_token_ids) > 0
+                or self.token_mask is not None)
 
 
 @dataclass
@@ -223,6 +245,7 @@ class InferenceModel:
         from ..parallel.tp import TPContext
         self.tp = tp_ctx if tp_ctx is not None else TPContext(None)
         tp = self.tp.size
+        self.adapters: Optional[AdapterPool] = None
         if cfg.arch == "gpt2":
             assert tp == 1, "gpt2 engine is the CPU plumbing tier (tp=1)"
             self._init_gpt2(cfg, device, dtype)
@@ -323,11 +346,13 @@ class InferenceModel:
     @torch.no_grad()
     def forward_tokens(self, token_ids: torch.Tensor, positions: torch.Tensor,
                        kv: PagedKVCache, slot_mapping: torch.Tensor,
-                       attn_fn, rows: Optional[torch.Tensor] = None
+                       attn_fn, rows: Optional[torch.Tensor] = None,
+                       adapter_index: Optional[torch.Tensor] = None
                        ) -> torch.Tensor:
         """Shared trunk: embed -> L x (norm, qkv, rope, kv-append, attn(fn),
         o-proj, norm, mlp) -> final norm.  Returns hidden (N, H), or of the
-        tokens that ``rows`` names."""
+        tokens that ``rows`` names.  ``adapter_index`` (N,) int32: the adapter
+        of every token, -1 for none."""
         if self.cfg.arch == "gpt2":
             hidden = self._forward_tokens_gpt2(token_ids, positions, kv,
                                                slot_mapping, attn_fn)
@@ -350,6 +375,13 @@ class InferenceModel:
         # (outputs of 1024: 3072 and 4096 rows +4 and +1%, 8192 -5; of 4096, 1300 and
         # 2048 rows +2 and -2, 6145 -4)
         adds = tp == 1 and residual.numel() >= 1 << 22
+        # every projection's adapters, by one grouping of the step's rows
+        plan = None if adapter_index is None else \
+            self.adapters.plan(adapter_index)
+
+        def adapt(li, proj, y, x):
+            if plan is not None:
+                self.adapters.add(li, proj, y, x, plan)
         for li, lw in enumerate(self.layers):
             if hidden is None:                        # (the residual has it)
                 hidden = ops.rmsnorm(residual, lw.input_ln, cfg.rms_norm_eps)
@@ -359,6 +391,7 @@ class InferenceModel:
             qkv = _mm_nt(hidden, lw.wqkv)
             if lw.bqkv is not None:
                 qkv = qkv + lw.bqkv
+            adapt(li, "qkv", qkv, hidden)
             # strided head views into the fused qkv row (no copies: the
             # rope + kv-append and attention kernels take a free token stride)
             q = qkv.narrow(1, 0, Hq * D).unflatten(1, (Hq, D))
@@ -373,20 +406,34 @@ class InferenceModel:
                     return x.new_empty(0, x.shape[1])
                 attn_out = attn_out.index_select(0, rows)
                 residual = residual.index_select(0, rows)
+                if plan is not None:
+                    plan = self.adapters.plan(
+                        adapter_index.index_select(0, rows))
             if adds and not few and _takes_rows(attn_out, lw.wo):
                 ops.linear_rows_add(residual, attn_out, lw.wo)
+                adapt(li, "o", residual, attn_out)
                 hidden = ops.rmsnorm(residual, lw.post_ln, cfg.rms_norm_eps)
             else:
                 hidden = _mm_nt(attn_out, lw.wo, not few)
+                adapt(li, "o", hidden, attn_out)
                 self.tp.all_reduce_(hidden)           # col-parallel o_proj
                 hidden, residual = ops.fused_add_rmsnorm(
                     hidden, residual, lw.post_ln, cfg.rms_norm_eps)
-            act = _gate_up(hidden, lw.w_gate_up, not few)
+            if plan is None:
+                act = _gate_up(hidden, lw.w_gate_up, not few)
+            else:                       # the adapters come before the activation
+                gate_up = _mm_nt(hidden, lw.w_gate_up, not few)
+                adapt(li, "gate_up", gate_up, hidden)
+                i = gate_up.shape[1] // 2
+                act = ops.silu_mul(gate_up.narrow(1, 0, i),
+                                   gate_up.narrow(1, i, i))
             if adds and not few and _takes_rows(act, lw.w_down):
                 ops.linear_rows_add(residual, act, lw.w_down)
+                adapt(li, "down", residual, act)
                 hidden = None
             else:
                 hidden = _mm_nt(act, lw.w_down, not few)
+                adapt(li, "down", hidden, act)
                 self.tp.all_reduce_(hidden)           # col-parallel down_proj
         # final residual add + norm (fused; residual buffer is dead after)
         if hidden is None:
@@ -442,10 +489,15 @@ class Engine:
                  tp_ctx=None,
                  seed: int = 0,
                  enable_radix_cache: bool = False,
-                 kv_token_capacity: Optional[int] = None):
+                 kv_token_capacity: Optional[int] = None,
+                 max_adapters: int = 8,
+                 max_adapter_rank: int = 64):
         self.cfg = cfg
         self.device = device
         self.dtype = dtype
+        # adapter slots (their memory is taken when the first one is loaded)
+        self.max_adapters = max_adapters
+        self.max_adapter_rank = max_adapter_rank
         # hybrid decoders (recurrent / state-space / latent-attention
         # layers): paged latent rows + per-sequence state slots, and one
         # mixed batch per step instead of a prefill and a decode pass
@@ -463,6 +515,8 @@ class Engine:
         self.max_model_len = max_model_len or cfg.max_position_embeddings
         self.states: Optional[StateSlots] = None
         self._forced: Dict[str, Request] = {}
+        self.rules = RequestRules(cfg.vocab_size, self.max_model_len + 1,
+                                  max_running_requests, device)
         if self.hybrid:
             self._init_hybrid(page_size, kv_bytes_budget, kv_token_capacity,
                               seed, decode_chunk_size)
@@ -555,9 +609,54 @@ class Engine:
         self._graph_seen: Dict[int, int] = {}
 
     # ------------------------------------------------------------ public API
+    def load_adapter(self, name: str, state_dict: Dict[str, torch.Tensor],
+                     scaling: float = 1.0):
+        """A low-rank adapter that requests may name (``SamplingParams.adapter``):
+        tensors as of ``models.lora.export_adapter``, B A times ``scaling`` on top of
+        the base weights.  Replaces one of the same name that no request uses."""
+        if self.hybrid or self.cfg.arch == "gpt2":
+            raise ValueError("adapters are for the llama and qwen2 families")
+        self._adapter_idle(name)
+        if self.model.adapters is None:
+            self.model.adapters = AdapterPool(self.model, self.max_adapters,
+                                              self.max_adapter_rank)
+        self.model.adapters.load(name, state_dict, scaling)
+
+    def unload_adapter(self, name: str):
+        if name not in self.adapters:
+            raise ValueError(f"no adapter {name!r}")
+        self._adapter_idle(name)
+        self.model.adapters.unload(name)
+
+    @property
+    def adapters(self) -> List[str]:
+        """Names of the loaded adapters."""
+        pool = getattr(self.model, "adapters", None)
+        return [] if pool is None else list(pool.names)
+
+    def _adapter_idle(self, name: str):
+        for r in self.running + self.waiting:
+            if r.sampling.adapter == name:
+                raise RuntimeError(f"adapter {name!r} is in use by {r.rid}")
+
+    def check_sampling(self, sampling: SamplingParams, input_ids: List[int]):
+        """ValueError for an adapter that is not loaded or rules that cannot hold
+        (:meth:`add_request` calls it)."""
+        if sampling.adapter and sampling.adapter not in self.adapters:
+            raise ValueError(f"no adapter {sampling.adapter!r}")
+        if sampling.has_rules:
+            self.rules.check(sampling, len(input_ids))
+
+    def _adapter_slots(self, reqs: List[Request]) -> Optional[List[int]]:
+        """Adapter slots of requests, None if none has one."""
+        if not any(r.sampling.adapter for r in reqs):
+            return None
+        return self.model.adapters.index(r.sampling.adapter for r in reqs)
+
     def add_request(self, rid: str, input_ids: List[int],
                     sampling: SamplingParams):
         assert len(input_ids) > 0
+        self.check_sampling(sampling, input_ids)
         req = Request(rid=rid, input_ids=list(input_ids), sampling=sampling,
                       arrival_t=time.time())
         self.waiting.append(req)
@@ -573,6 +672,7 @@ class Engine:
         copied per child so decode writes never touch shared pages).
         Child rids are '<prefix>-s0' .. '<prefix>-s<n-1>'."""
         assert n >= 1
+        self.check_sampling(sampling, input_ids)
         if n == 1 or not self.enable_prefix_sharing:
             for s_ in range(n):
                 self.add_request(f"{rid_prefix}-s{s_}", input_ids, sampling)
@@ -685,7 +785,9 @@ class Engine:
             nxt = self.waiting[0]
             radix_pages: List[int] = []
             radix_len = 0
-            if self.radix is not None and nxt.prefill_pos == 0:
+            # (an adapter's keys and values are its own: no shared prefixes)
+            if self.radix is not None and nxt.prefill_pos == 0 \
+                    and not nxt.sampling.adapter:
                 radix_pages, radix_len = self.radix.match(nxt.input_ids)
             need = min(len(nxt.input_ids) - nxt.prefill_pos - radix_len,
                        admit_budget)
@@ -807,13 +909,15 @@ class Engine:
 
     def _emit(self, r: Request) -> RequestOutput:
         sid = self._seq_ids.pop(r.rid, None)
+        self.rules.release(r.rid)
         if sid is not None:
             # Aborted requests (weight-update time-box) must NOT donate KV
             # to the radix cache: they are emitted on the step AFTER
             # flush_radix(), so their pages hold OLD-weight KV and a
             # token-exact continuation of the same request would radix-match
             # that stale prefix and skip recomputing it under new weights.
-            if self.radix is not None and r.finish_reason != "abort":
+            if self.radix is not None and r.finish_reason != "abort" \
+                    and not r.sampling.adapter:
                 written = self.kv.seq_len(sid)   # last sampled token has no KV
                 toks = (r.input_ids + r.output_ids)[:written]
                 self.radix.insert(toks, self.kv._seq_pages.get(sid, []))
@@ -852,7 +956,8 @@ class Engine:
         no_filter = all(
             (r.sampling.top_k <= 0 or r.sampling.top_k >= logits.shape[-1])
             and r.sampling.top_p >= 1.0 for r in reqs)
-        tokens, lps = ops.sample(logits, temp, tk, tp, seed,
+        tokens, lps = self._draw(logits, temp, tk, tp, seed,
+                                 self.rules.rows(reqs),
                                  generator=self._gen, no_filter=no_filter)
         tokens_l = tokens.tolist()
         lps_l = lps.tolist()
@@ -869,6 +974,27 @@ class Engine:
             elif r.seq_len >= self.max_model_len:
                 r.finished = True
                 r.finish_reason = "length"
+            self._next_mask(r)
+
+    def _draw(self, logits, temp, tk, tp, seed, rows, **kw):
+        """``ops.sample`` under the rules of the requests whose slots ``rows`` names (None:
+        no request has any), the drawn tokens in their histories.  Their
+        log-probabilities are the model's own, as all others'."""
+        if rows is None:
+            return ops.sample(logits, temp, tk, tp, seed, **kw)
+        table = self.rules.table
+        tokens, lps = ops.sample(ops.adjust_logits(logits, table, rows), temp,
+                                 tk, tp, seed, **kw)
+        lps.copy_(torch.where(rows >= 0, ops.gather_logprobs(logits, tokens),
+                              lps))
+        ops.append_tokens(table, rows, tokens)
+        return tokens, lps
+
+    def _next_mask(self, r: Request):
+        if r.sampling.token_mask is not None and not r.finished \
+                and not self.rules.advance(r):
+            r.finished = True
+            r.finish_reason = "stop"
 
     # ----------------------------------------------------- hybrid decoders
     def _hybrid_batch(self, items):
@@ -1112,8 +1238,12 @@ class Engine:
             parts.append(np.concatenate(
                 [self.kv.slots_for_host(sid, 0, s + m)
                  for sid, s, m in zip(sids, starts, lens)]))
+        own = self._adapter_slots(reqs)
+        if own is not None:
+            parts.append(np.repeat(np.asarray(own, np.int32), lens))
         tokens, positions, slots, cu_q_t, cu_k_t, rows_t, *hist = \
             self._upload(parts)
+        index = None if own is None else hist.pop()
 
         def attn_fn(li, q, k, v):
             if not fresh:
@@ -1124,7 +1254,7 @@ class Engine:
                                                 self._scale, causal=True)
 
         return self.model.forward_tokens(tokens.long(), positions, self.kv,
-                                         slots, attn_fn, rows_t)
+                                         slots, attn_fn, rows_t, index)
 
     def _upload(self, parts) -> List[torch.Tensor]:
         """int32 arrays as device tensors, through one pinned buffer and one
@@ -1204,9 +1334,10 @@ class Engine:
     def _decode_chunk_len(self, reqs: List[Request]) -> int:
         """How many decode iterations can run device-side without a host
         sync: bounded by the chunk size, every request's remaining token
-        budget, and the model-len fence.  Stop-token requests decode 1 at a
-        time (token-exact stop)."""
-        if any(r.sampling.stop_token_ids for r in reqs):
+        budget, and the model-len fence.  Stop-token and token-mask requests decode
+        1 at a time (token-exact stop, a mask for every token)."""
+        if any(r.sampling.stop_token_ids or r.sampling.token_mask is not None
+               for r in reqs):
             return 1
         rem = min(r.sampling.max_new_tokens - len(r.output_ids) for r in reqs)
         rem = min(rem, min(self.max_model_len - r.seq_len for r in reqs))
@@ -1259,6 +1390,10 @@ class Engine:
         no_filter = all(
             (r.sampling.top_k <= 0 or r.sampling.top_k >= self.cfg.vocab_size)
             and r.sampling.top_p >= 1.0 for r in reqs)
+        rule_rows = self.rules.rows(reqs)
+        own = self._adapter_slots(reqs)
+        index = None if own is None else torch.tensor(
+            own, dtype=torch.int32, device=dev)
         out_tokens = torch.empty(C, B, dtype=torch.int64, device=dev)
         out_lps = torch.empty(C, B, dtype=torch.float32, device=dev)
 
@@ -1269,7 +1404,7 @@ class Engine:
             try:
                 self._decode_graphed(B, C, tokens, pos0, slots_all,
                                      page_table, temp, tk, tp, seed0,
-                                     out_tokens, out_lps)
+                                     out_tokens, out_lps, rule_rows, index)
                 C_done = True
             except Exception as e:
                 import traceback
@@ -1288,11 +1423,12 @@ class Engine:
 
             for s in range(C):
                 positions = pos0 + s
-                hidden = self.model.forward_tokens(tokens, positions, self.kv,
-                                                   slots_all[s], attn_fn)
+                hidden = self.model.forward_tokens(
+                    tokens, positions, self.kv, slots_all[s], attn_fn,
+                    adapter_index=index)
                 logits = self.model.logits(hidden)
-                tokens, lps = ops.sample(logits, temp, tk, tp, seed0 + s,
-                                         generator=self._gen,
+                tokens, lps = self._draw(logits, temp, tk, tp, seed0 + s,
+                                         rule_rows, generator=self._gen,
                                          no_filter=no_filter)
                 out_tokens[s] = tokens
                 out_lps[s] = lps
@@ -1321,7 +1457,8 @@ class Engine:
         return int(self.kv.slots_for(self._SCRATCH_SEQ, 0, 1)[0])
 
     def _decode_graphed(self, B, C, tokens, pos0, slots_all, page_table,
-                        temp, tk, tp, seed0, out_tokens, out_lps):
+                        temp, tk, tp, seed0, out_tokens, out_lps,
+                        rule_rows=None, index=None):
         """hipGraph decode: capture one decode iteration per batch size and
         replay it per token.  All state (tokens/positions/ctx/slots/page
         table/seed) lives in static device buffers; positions, ctx and the
@@ -1332,7 +1469,14 @@ class Engine:
         # [B:Bb) are dummies writing KV into a reserved scratch slot
         Bb = decode_bucket(B) if self._decode_buckets else B
         scratch = self._decode_scratch_slot() if Bb > B else 0
-        st = self._graphs.get(Bb)
+        # steps with rules or adapters are captured apart from those without, and anew
+        # when the rules' tables were made larger
+        key = Bb if rule_rows is None and index is None else \
+            (Bb, rule_rows is not None, index is not None)
+        st = self._graphs.get(key)
+        if st is not None and rule_rows is not None \
+                and st["rules"] is not self.rules.table:
+            st = None
         if st is None:
             st = {
                 "tokens": torch.zeros(Bb, dtype=torch.int64, device=dev),
@@ -1348,7 +1492,11 @@ class Engine:
                 "seed": torch.zeros(1, dtype=torch.int64, device=dev),
                 "out_t": torch.zeros(Bb, dtype=torch.int64, device=dev),
                 "out_l": torch.zeros(Bb, dtype=torch.float32, device=dev),
+                "rules": None if rule_rows is None else self.rules.table,
             }
+            none = lambda t: None if t is None else torch.full(
+                (Bb,), -1, dtype=torch.int32, device=dev)
+            st["rows"], st["index"] = none(rule_rows), none(index)
             if Bb > B:
                 st["ptab"].fill_(scratch // self.kv.page_size)
 
@@ -1358,10 +1506,11 @@ class Engine:
                         q, self.kv.k_cache[li], self.kv.v_cache[li],
                         st["ptab"], st["ctx"], self._scale)
                 hidden = self.model.forward_tokens(
-                    st["tokens"], st["pos"], self.kv, st["slots"], attn_fn)
+                    st["tokens"], st["pos"], self.kv, st["slots"], attn_fn,
+                    adapter_index=st["index"])
                 logits = self.model.logits(hidden)
-                ops.sample(logits, st["temp"], st["tk"], st["tp"], 0,
-                           no_filter=True, seed_dev=st["seed"],
+                self._draw(logits, st["temp"], st["tk"], st["tp"], 0,
+                           st["rows"], no_filter=True, seed_dev=st["seed"],
                            out=(st["out_t"], st["out_l"]))
                 st["tokens"].copy_(st["out_t"])
                 st["pos"] += 1
@@ -1380,10 +1529,20 @@ class Engine:
             mp = min(page_table.shape[1], self._graph_max_pages)
             st["ptab"][:B].zero_()
             st["ptab"][:B, :mp].copy_(page_table[:, :mp])
-            with torch.cuda.stream(side):
-                for _ in range(2):
-                    body()
-            torch.cuda.current_stream().wait_stream(side)
+            if index is not None:
+                st["index"][:B].copy_(index)
+            if rule_rows is not None:
+                st["rows"][:B].copy_(rule_rows)
+                lens = st["rules"].total_len.clone()
+            side.wait_stream(torch.cuda.current_stream())
+            try:
+                with torch.cuda.stream(side):
+                    for _ in range(2):
+                        body()
+            finally:
+                torch.cuda.current_stream().wait_stream(side)
+                if rule_rows is not None:   # (the warm-up's tokens are none)
+                    st["rules"].total_len.copy_(lens)
             g = torch.cuda.CUDAGraph()
             if self._graph_pool is None:
                 with torch.cuda.graph(g):
@@ -1393,7 +1552,7 @@ class Engine:
                 with torch.cuda.graph(g, pool=self._graph_pool):
                     body()
             st["graph"] = g
-            self._graphs[Bb] = st
+            self._graphs[key] = st
 
         # load chunk state into the static buffers
         st["tokens"][:B].copy_(tokens)
@@ -1406,7 +1565,14 @@ class Engine:
         st["tk"][:B].copy_(tk)
         st["tp"][:B].copy_(tp)
         st["seed"].fill_(seed0)
+        if index is not None:
+            st["index"][:B].copy_(index)
+        if rule_rows is not None:
+            st["rows"][:B].copy_(rule_rows)
         if Bb > B:
+            for name in ("rows", "index"):
+                if st[name] is not None:
+                    st[name][B:].fill_(-1)
             # reset dummy rows (a previous call on this bucket with a
             # larger real B may have left real state here): KV writes go
             # to the scratch slot, attention reads ctx=1 from the zeroed
@@ -1441,3 +1607,4 @@ class Engine:
                 elif r.seq_len >= self.max_model_len:
                     r.finished = True
                     r.finish_reason = "length"
+            self._next_mask(r)

@@ -96,8 +96,12 @@ class EngineRunner:
             rid = f"r{self._rid_counter}"
         fut = loop.create_future()
         self._futures[rid] = (loop, fut)
-        with self._admin_lock():
-            self.engine.add_request(rid, input_ids, sp)
+        try:
+            with self._admin_lock():
+                self.engine.add_request(rid, input_ids, sp)
+        except ValueError:               # refused: nobody will answer
+            self._futures.pop(rid, None)
+            raise
         self.start()
         self._wake.set()
         return fut
@@ -116,8 +120,13 @@ class EngineRunner:
             fut = loop.create_future()
             self._futures[f"{prefix}-s{s_}"] = (loop, fut)
             futs.append(fut)
-        with self._admin_lock():
-            self.engine.add_request_group(prefix, input_ids, sp, n)
+        try:
+            with self._admin_lock():
+                self.engine.add_request_group(prefix, input_ids, sp, n)
+        except ValueError:
+            for s_ in range(n):
+                self._futures.pop(f"{prefix}-s{s_}", None)
+            raise
         self.start()
         self._wake.set()
         return futs
@@ -154,6 +163,15 @@ class EngineRunner:
                 "#queue_req": self.engine.num_queued(),
                 "last_gen_throughput": self.throughput,
                 "weight_version": self.weight_version}
+
+    def load_adapter(self, name: str, state_dict, scaling: float = 1.0):
+        """``Engine.load_adapter`` under the step lock."""
+        with self._admin_lock():
+            self.engine.load_adapter(name, state_dict, scaling)
+
+    def unload_adapter(self, name: str):
+        with self._admin_lock():
+            self.engine.unload_adapter(name)
 
     def update_weights(self, state_dict, version: int, strict: bool = False,
                        abort_in_flight: bool = True):

@@ -40,7 +40,16 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
             top_k=int(d.get("top_k", -1)),
             top_p=float(d.get("top_p", 1.0)),
             max_new_tokens=int(d.get("max_new_tokens", 128)),
-            stop_token_ids=tuple(d.get("stop_token_ids", ())))
+            stop_token_ids=tuple(d.get("stop_token_ids", ())),
+            repetition_penalty=float(d.get("repetition_penalty", 1.0)),
+            frequency_penalty=float(d.get("frequency_penalty", 0.0)),
+            presence_penalty=float(d.get("presence_penalty", 0.0)),
+            # {"token": value}; JSON has no -inf, its clients write "-inf"
+            logit_bias=tuple((int(t), float(v)) for t, v in
+                             (d.get("logit_bias") or {}).items()),
+            allowed_token_ids=tuple(
+                int(t) for t in d.get("allowed_token_ids") or ()),
+            adapter=str(d.get("adapter") or ""))
 
     def _meta(o, include_logprobs: bool) -> dict:
         m = {"finish_reason": {"type": o.finish_reason},
@@ -60,7 +69,10 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
         want_lp = bool(body.get("return_logprob", False))
         stream = bool(body.get("stream", False))
 
-        futs = runner.submit_group(input_ids, sp, n)
+        try:
+            futs = runner.submit_group(input_ids, sp, n)
+        except ValueError as e:          # no such adapter, impossible rules
+            return JSONResponse({"success": False, "message": str(e)}, 400)
 
         if not stream:
             outs = await asyncio.gather(*futs)
@@ -116,6 +128,47 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
         # prefix cache — drop it
         engine.flush_radix()
         return {"status": "ok"}
+
+    @app.post("/load_adapter")
+    async def load_adapter(request: Request):
+        """A low-rank adapter that requests name in ``sampling_params.adapter``:
+        {"name": N, "path": "/node/local/adapter.safetensors", "scaling": S} or raw
+        safetensors bytes with X-Adapter-Name and X-Adapter-Scaling headers."""
+        if not _sender_ok(request):
+            return JSONResponse({"success": False,
+                                 "message": "sender not in allowed CIDRs"},
+                                403)
+        from safetensors.torch import load, load_file
+        if request.headers.get("content-type", "").startswith(
+                "application/json"):
+            body = await request.json()
+            name, scaling = str(body["name"]), float(body.get("scaling", 1.0))
+            read = lambda: load_file(body["path"])
+        else:
+            raw = await request.body()
+            name = request.headers.get("x-adapter-name", "")
+            scaling = float(request.headers.get("x-adapter-scaling", "1.0"))
+            read = lambda: load(raw)
+        try:
+            await asyncio.get_running_loop().run_in_executor(
+                None, lambda: runner.load_adapter(name, read(), scaling))
+        except (ValueError, RuntimeError, OSError) as e:
+            return JSONResponse({"success": False, "message": str(e)}, 400)
+        return {"success": True, "adapters": engine.adapters}
+
+    @app.post("/unload_adapter")
+    async def unload_adapter(request: Request):
+        if not _sender_ok(request):
+            return JSONResponse({"success": False,
+                                 "message": "sender not in allowed CIDRs"},
+                                403)
+        body = await request.json()
+        try:
+            await asyncio.get_running_loop().run_in_executor(
+                None, lambda: runner.unload_adapter(str(body["name"])))
+        except (ValueError, RuntimeError) as e:
+            return JSONResponse({"success": False, "message": str(e)}, 400)
+        return {"success": True, "adapters": engine.adapters}
 
     @app.post("/update_weights_from_agent")
     async def update_weights_from_agent(request: Request):
@@ -326,6 +379,9 @@ def main():
                         "serving; RL trainers flush it every publish)")
     p.add_argument("--no-radix-cache", dest="radix_cache",
                    action="store_false")
+    p.add_argument("--max-adapters", type=int, default=8,
+                   help="adapters that /load_adapter may hold at a time")
+    p.add_argument("--max-adapter-rank", type=int, default=64)
     p.add_argument("--allowed-sender-cidrs", default=None,
                    help="comma-separated CIDRs allowed to push weights "
                         "(reference: allowed_sender_ips)")
@@ -340,14 +396,18 @@ def main():
         from ..rollout.loader import engine_from_dir
         engine = engine_from_dir(args.model, device=device, dtype=dtype,
                                  kv_bytes_budget=int(args.kv_gb * (1 << 30)),
-                                 enable_radix_cache=args.radix_cache)
+                                 enable_radix_cache=args.radix_cache,
+                                 max_adapters=args.max_adapters,
+                                 max_adapter_rank=args.max_adapter_rank)
         cfg = engine.cfg
         args.load = False
     else:
         cfg = get_model_config(args.model)
         engine = Engine(cfg, device=device, dtype=dtype,
                         kv_bytes_budget=int(args.kv_gb * (1 << 30)),
-                        enable_radix_cache=args.radix_cache)
+                        enable_radix_cache=args.radix_cache,
+                        max_adapters=args.max_adapters,
+                        max_adapter_rank=args.max_adapter_rank)
     if args.load is False:
         pass
     elif args.load:

@@ -102,7 +102,8 @@ class StreamPPOTrainer:
         if arr.model.lora_rank > 0:
             from ..models.lora import apply_lora
             apply_lora(actor_model, arr.model.lora_rank,
-                       alpha=arr.model.lora_alpha)
+                       alpha=arr.model.lora_alpha,
+                       seeded_dropout=arr.model.lora_dropout)
         actor_pad_to = (arr.actor.ppo_max_token_len_per_gpu *
                         arr.actor.ulysses_sequence_parallel_size
                         if arr.actor.use_dynamic_bsz else 0)
