@@ -14,9 +14,9 @@
 // read A in every block of columns; h is 1% of y.)
 //
 // What bounds it: memory, prompts by y and out (6504 rows, ranks 32, the four projections of
-// 4096 / 6144 / 14336 numbers, 1.43 GB: 404 us, 3.5 TB/s; the widest, 746 MB, 170 us, where a
+// 4096 / 6144 / 14336 numbers, 1.43 GB: 363 us, 3.9 TB/s; the widest, 746 MB, 153 us, where a
 // copy of the same tiles takes 131), decode by the adapters (57 rows of as many adapters of
-// ranks 64 and 32, 0.45 GB: 152 us, 2.9 TB/s); one row by nine launches, 48 us.
+// ranks 64 and 32, 0.45 GB: 152 us, 2.9 TB/s); one row by nine launches, 41 us (34 in a graph).
 //
 // Matrix cores: 16x16x32 in bf16, 16x16x4 in fp32.  h is a sum in 32 bits; as an operand
 // in bf16 it is split in two bf16 numbers, h = hi + lo, each with its own product, so that what
@@ -476,7 +476,8 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
 // columns of a row, a 16-byte word, and 16 lanes 256 bytes of it: tile c's column i is
 // VEC * i + c.  b and h go through LDS, PRE ranks at a time, b's rows in the tiles' order.
 // (6504 rows of 28672 columns, rank 32: lanes by rows as above for few 220 us, so 185, with
-// registers for four blocks a CU 170; for five they spill, 363.  A wave that keeps its
+// registers for four blocks a CU 170, without spills, which h's shares in flight took, 153;
+// for five it spills, 373.  A wave that keeps its
 // columns of b and goes through the rows, their loads a round ahead, has too few of
 // them on their way: 243 to 345.)
 template <typename T, int PRE, bool WORDS, bool OUT_WORDS>
@@ -503,7 +504,7 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
   const float s = slot < 0 ? 0.f : scale[slot];
   const int mine = wid * 16 + lhi * 4;            // this lane's first row
   const bool whole = OUT_WORDS && n0 + COLS <= end;
-  long row[4];
+  int row[4];
   Word yv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) row[i] = order[min(mine + i, rows - 1)];
@@ -526,14 +527,18 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
       const int g = threadIdx.x + i * 256, r = g / (PRE / 4), j = j0 + g % (PRE / 4) * 4;
       hv[i] = {0.f, 0.f, 0.f, 0.f};
       if (r >= rows || j >= rank) continue;
-      hv[i] = shares_sum(hh + (uint32_t)(r * z.parts * z.rank16 + j), share, z.split);
+      const float* p = hh + (uint32_t)(r * z.parts * z.rank16 + j);
+      hv[i] = *reinterpret_cast<const f32x4_t*>(p);
+#pragma unroll 1
+      for (int w = 1; w < z.split; ++w)
+        hv[i] += *reinterpret_cast<const f32x4_t*>(p + w * share);
     }
   };
   fetch(0);
   if (whole)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      yv[i] = *reinterpret_cast<const Word*>(y + row[i] * z.ldy + n0 + l15 * VEC);
+      yv[i] = *reinterpret_cast<const Word*>(y + (long)row[i] * z.ldy + n0 + l15 * VEC);
   if (rank == 0 && out == y) return;
   f32x4_t acc[VEC];
 #pragma unroll
@@ -583,14 +588,14 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
       if (rank > 0)
 #pragma unroll
         for (int c = 0; c < VEC; ++c) w.v[c] = (T)((float)w.v[c] + acc[c][i]);
-      *reinterpret_cast<Word*>(out + row[i] * z.ldo + n0 + l15 * VEC) = w;
+      *reinterpret_cast<Word*>(out + (long)row[i] * z.ldo + n0 + l15 * VEC) = w;
     } else {
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
         const int n = n0 + l15 * VEC + c;
         if (n >= end) break;
-        const T old = y[row[i] * z.ldy + n];
-        out[row[i] * z.ldo + n] = rank > 0 ? (T)((float)old + acc[c][i]) : old;
+        const T old = y[(long)row[i] * z.ldy + n];
+        out[(long)row[i] * z.ldo + n] = rank > 0 ? (T)((float)old + acc[c][i]) : old;
       }
     }
   }
@@ -629,11 +634,12 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
   auto stream = at::hip::getCurrentHIPStream();
   const int* pl = plan.data_ptr<int>();
   // Tiles of ranks that a block takes: all of them in equal groups of up to three or four
-  // Up to 1024 rows a block takes 16 of them in 16 waves, else 32 in 8: of few rows there
+  // Up to 1024 rows a block takes 16 of them in 16 waves, else 32 in 4: of few rows there
   // are too few blocks otherwise, of many each one reads A again (620 rows, fp32, 8960 -> 20
   // 21 us in blocks of 32 rows and 16 of 16; 6504 rows, bf16, 14336 -> 32, before the
-  // loads were dealt as they are, 72 and 97).
-  const int sixteens = tile_rows(z.T) / 16, RT = z.T <= 1024 ? 1 : 2, NW = 16 / RT;
+  // loads were dealt as they are, 72 and 97; since then, four projections of those rows, 132
+  // in blocks of 8 waves and 125 of 4).
+  const int sixteens = tile_rows(z.T) / 16, RT = z.T <= 1024 ? 1 : 2, NW = RT == 1 ? 16 : 4;
   const int subs = sixteens / RT;
   // Tiles of ranks that a block takes: all of them in equal groups, of up to two where a wave
   // of 16 has 128 registers (three spill: 128 rows, 3 x 16 ranks of 4096, 8.0 us and 6.5 by
@@ -661,7 +667,7 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
     down(adapter_down_kernel<T, N, R, C, W>, N);
 #define DOWNS(N, R, C) DOWN(N, R, C, true) DOWN(N, R, C, false)
   DOWNS(16, 1, 1) DOWNS(16, 1, 2)
-  DOWNS(8, 2, 1) DOWNS(8, 2, 2) DOWNS(8, 2, 3) DOWNS(8, 2, 4)
+  DOWNS(4, 2, 1) DOWNS(4, 2, 2) DOWNS(4, 2, 3) DOWNS(4, 2, 4)
 #undef DOWNS
 #undef DOWN
   HIP_CHECK_KERNEL();
@@ -686,9 +692,19 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
   HIP_CHECK_KERNEL();
 }
 
-void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Tensor a,
-                 torch::Tensor b, torch::Tensor scale, torch::Tensor ranks,
-                 torch::Tensor plan, int64_t slots, std::vector<int64_t> widths) {
+torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
+                          const torch::Tensor& a, const torch::Tensor& b,
+                          const torch::Tensor& scale,
+                          const c10::optional<torch::Tensor>& ranks,
+                          const torch::Tensor& plan, int64_t slots,
+                          std::vector<int64_t> widths,
+                          const c10::optional<torch::Tensor>& into) {
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(y.requires_grad() || x.requires_grad() || a.requires_grad() ||
+                    b.requires_grad() || scale.requires_grad()),
+              "adapter_add has no gradients: call it under torch.no_grad()");
+  torch::Tensor out = into.has_value() ? *into : torch::empty(y.sizes(), y.options());
+  if (widths.empty() && y.dim() == 2) widths.push_back(y.size(1));
   TORCH_CHECK(y.is_cuda() && y.dim() == 2 && x.dim() == 2 && a.dim() == 4 &&
                   b.dim() == 3 && out.sizes() == y.sizes(),
               "adapter_add: y, out (T, N), x (T, K), a (S, P, r, K), b (S, N, r)");
@@ -710,9 +726,9 @@ void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Ten
   TORCH_CHECK(scale.device() == y.device() && scale.scalar_type() == torch::kFloat32 &&
                   scale.is_contiguous() && scale.numel() == S,
               "adapter_add: scale (S) fp32");
-  const bool some = ranks.defined() && ranks.numel() > 0;
-  TORCH_CHECK(!some || (ranks.device() == y.device() && ranks.is_contiguous() &&
-                        ranks.scalar_type() == torch::kInt32 && ranks.numel() == S),
+  const bool some = ranks.has_value();
+  TORCH_CHECK(!some || (ranks->device() == y.device() && ranks->is_contiguous() &&
+                        ranks->scalar_type() == torch::kInt32 && ranks->numel() == S),
               "adapter_add: ranks (S) int32");
   Shape z{};
   z.T = (int)T, z.K = (int)K, z.N = (int)N, z.parts = (int)widths.size();
@@ -733,10 +749,10 @@ void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Ten
     z.first[p + 1] = z.first[p] + (int)widths[p];
   }
   TORCH_CHECK(z.first[widths.size()] == N, "adapter_add: widths that do not add up to N");
-  if (T == 0 || N == 0) return;
+  if (T == 0 || N == 0) return out;
   const bool words_down = whole(x, z.ldx) && whole(a, K), words_up = whole(b, r);
   const c10::DeviceGuard guard(y.device());
-  const int* rk = some ? ranks.data_ptr<int>() : nullptr;
+  const int* rk = some ? ranks->data_ptr<int>() : nullptr;
   if (y.scalar_type() == torch::kBFloat16)
     launch_adapter_add<__bf16>(out, y, x, a, b, scale, rk, plan, z, words_down, words_up,
                        words_out);
@@ -745,4 +761,5 @@ void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Ten
                        words_out);
   else
     TORCH_CHECK(false, "adapter_add: dtype must be bf16 or fp32");
+  return out;
 }

@@ -103,9 +103,13 @@ void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
 void append_tokens(torch::Tensor history, torch::Tensor total_len, torch::Tensor rows,
                    torch::Tensor tokens);
 torch::Tensor adapter_plan(torch::Tensor index, int64_t slots);
-void adapter_add(torch::Tensor out, torch::Tensor y, torch::Tensor x, torch::Tensor a,
-                 torch::Tensor b, torch::Tensor scale, torch::Tensor ranks,
-                 torch::Tensor plan, int64_t slots, std::vector<int64_t> widths);
+torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
+                          const torch::Tensor& a, const torch::Tensor& b,
+                          const torch::Tensor& scale,
+                          const c10::optional<torch::Tensor>& ranks,
+                          const torch::Tensor& plan, int64_t slots,
+                          std::vector<int64_t> widths,
+                          const c10::optional<torch::Tensor>& into);
 void varlen_attention_backward_v3(
     torch::Tensor dq, torch::Tensor dk, torch::Tensor dv,
     torch::Tensor q, torch::Tensor k, torch::Tensor v,

@@ -13,6 +13,7 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
+import polyrl_amd.ops as _ops
 from . import ref
 
 MOST_TOKENS = (1 << 19) - 1      # of a history
@@ -141,8 +142,7 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, rows: torch.Tensor,
     if rows.dtype != torch.int32 or rows.shape != logits.shape[:1]:
         raise ValueError("adjust_logits: rows (N,) int32")
     if logits.is_cuda:
-        from . import _require_ext
-        ext = _require_ext()
+        ext = _ops._require_ext()
         if out is None:
             out = torch.empty(logits.shape, dtype=logits.dtype,
                               device=logits.device)
@@ -163,8 +163,7 @@ def append_tokens(rules: LogitRules, rows: torch.Tensor,
             or tokens.dtype != torch.int64 or tokens.shape != rows.shape:
         raise ValueError("append_tokens: rows (N,) int32, tokens (N,) int64")
     if rows.is_cuda:
-        from . import _require_ext
-        _require_ext().append_tokens(rules.history, rules.total_len,
-                                     rows.contiguous(), tokens.contiguous())
+        _ops._require_ext().append_tokens(rules.history, rules.total_len,
+                                          rows.contiguous(), tokens.contiguous())
         return
     ref.append_tokens(rules, rows, tokens)
