@@ -55,15 +55,14 @@ template <> struct Operand<float> {
 };
 
 // p[0 .. have) of a lane's numbers, zeros behind.  WORDS: 16 bytes at p can be read
-// wherever have > 0.  ONCE: nobody else reads them
-template <typename T, bool WORDS, bool ONCE = false>
+// wherever have > 0
+template <typename T, bool WORDS>
 DEV_INLINE i32x4_t load_some(const T* p, int have) {
   constexpr int PER = Operand<T>::PER;
   if (have <= 0) return i32x4_t{0, 0, 0, 0};
   T v[PER];
   if (WORDS) {
-    const i32x4_t* at = reinterpret_cast<const i32x4_t*>(p);
-    const i32x4_t w = ONCE ? __builtin_nontemporal_load(at) : *at;
+    const i32x4_t w = *reinterpret_cast<const i32x4_t*>(p);
     if (have >= PER) return w;
     __builtin_memcpy(v, &w, 16);
   } else {
@@ -180,12 +179,6 @@ struct Shape {
   int first[9];                       // columns of the parts
 };
 
-#ifndef MOST_REPS
-#define MOST_REPS 16
-#endif
-#ifndef UP_BLOCKS
-#define UP_BLOCKS 2048
-#endif
 constexpr int MOST_SPLIT = 4;
 
 // Operand tiles from rows that lie far apart.  The matrix cores want row l % 16 in lane l,
@@ -508,8 +501,8 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
   Word yv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) row[i] = order[min(mine + i, rows - 1)];
-  constexpr int NB = COLS * GRAN / (256);     // words of b that a thread brings
-  constexpr int NH = 64 * PRE / 4 / (256);
+  constexpr int NB = COLS * GRAN / 256;           // words of b that a thread brings
+  constexpr int NH = 64 * PRE / 4 / 256;
   const long share = (long)z.T * z.parts * z.rank16;
   const T* bb = b + ((long)max(slot, 0) * z.N + n0) * z.rank;
   const float* hh = h + ((long)place * z.parts + at.part) * z.rank16;
@@ -633,7 +626,6 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
                                bool words_down, bool words_up, bool words_out) {
   auto stream = at::hip::getCurrentHIPStream();
   const int* pl = plan.data_ptr<int>();
-  // Tiles of ranks that a block takes: all of them in equal groups of up to three or four
   // Up to 1024 rows a block takes 16 of them in 16 waves, else 32 in 4: of few rows there
   // are too few blocks otherwise, of many each one reads A again (620 rows, fp32, 8960 -> 20
   // 21 us in blocks of 32 rows and 16 of 16; 6504 rows, bf16, 14336 -> 32, before the
@@ -696,7 +688,7 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                           const torch::Tensor& a, const torch::Tensor& b,
                           const torch::Tensor& scale,
                           const c10::optional<torch::Tensor>& ranks,
-                          const torch::Tensor& plan, int64_t slots,
+                          const torch::Tensor& plan, int64_t rows, int64_t slots,
                           std::vector<int64_t> widths,
                           const c10::optional<torch::Tensor>& into) {
   TORCH_CHECK(!at::GradMode::is_enabled() ||
@@ -720,8 +712,9 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                 "adapter_add: tensors of one type and device");
   for (const auto& t : {out, y, x})
     TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, "adapter_add: rows of adjacent numbers");
-  TORCH_CHECK(out.data_ptr() != y.data_ptr() || out.strides() == y.strides(),
-              "adapter_add: out is y or apart from it");
+  TORCH_CHECK((out.data_ptr() != y.data_ptr() || out.strides() == y.strides()) &&
+                  (T <= 1 || out.stride(0) >= N),
+              "adapter_add: out is y or apart from it, its rows from each other");
   TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "adapter_add: contiguous a and b");
   TORCH_CHECK(scale.device() == y.device() && scale.scalar_type() == torch::kFloat32 &&
                   scale.is_contiguous() && scale.numel() == S,
@@ -736,19 +729,22 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
   z.ldx = x.stride(0), z.ldy = y.stride(0), z.ldo = out.stride(0);
   z.most = (int)most_tiles(T, S);
   TORCH_CHECK(plan.device() == y.device() && plan.scalar_type() == torch::kInt32 &&
-                  plan.numel() == PLAN_HEAD + 4L * z.most + T,
+                  rows == T && plan.numel() == PLAN_HEAD + 4L * z.most + T,
               "adapter_add: a plan of other rows");
   const long size = y.element_size();
   auto whole = [&](const torch::Tensor& t, long row) {
     return ((uintptr_t)t.data_ptr() & 15) == 0 && row * size % 16 == 0;
   };
   bool words_out = whole(out, z.ldo) && whole(y, z.ldy);
+  long left = N;
   for (size_t p = 0; p < widths.size(); ++p) {
-    TORCH_CHECK(widths[p] >= 0 && widths[p] <= N, "adapter_add: widths of the parts");
+    TORCH_CHECK(widths[p] >= 0 && widths[p] <= left,
+                "adapter_add: widths that do not add up to N");
+    left -= widths[p];
     words_out = words_out && z.first[p] * size % 16 == 0;
     z.first[p + 1] = z.first[p] + (int)widths[p];
   }
-  TORCH_CHECK(z.first[widths.size()] == N, "adapter_add: widths that do not add up to N");
+  TORCH_CHECK(left == 0, "adapter_add: widths that do not add up to N");
   if (T == 0 || N == 0) return out;
   const bool words_down = whole(x, z.ldx) && whole(a, K), words_up = whole(b, r);
   const c10::DeviceGuard guard(y.device());

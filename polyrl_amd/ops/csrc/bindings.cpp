@@ -107,7 +107,7 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                           const torch::Tensor& a, const torch::Tensor& b,
                           const torch::Tensor& scale,
                           const c10::optional<torch::Tensor>& ranks,
-                          const torch::Tensor& plan, int64_t slots,
+                          const torch::Tensor& plan, int64_t rows, int64_t slots,
                           std::vector<int64_t> widths,
                           const c10::optional<torch::Tensor>& into);
 void varlen_attention_backward_v3(

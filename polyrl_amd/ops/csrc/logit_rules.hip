@@ -267,6 +267,9 @@ void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
   TORCH_CHECK((V <= 1 || (logits.stride(1) == 1 && out.stride(1) == 1)) &&
                   V < (1L << 30),
               "adjust_logits: rows of adjacent numbers");
+  TORCH_CHECK((out.data_ptr() != logits.data_ptr() || out.strides() == logits.strides()) &&
+                  (N <= 1 || out.stride(0) >= V),
+              "adjust_logits: out is logits or apart from it, its rows from each other");
   for (const auto& t : {rows, history, prompt_len, total_len, bias_tokens, mask, masked})
     check_ints(t, logits, "adjust_logits");
   const long R = history.size(0), cap = history.size(1), nb = bias_tokens.size(1);
@@ -319,7 +322,7 @@ void append_tokens(torch::Tensor history, torch::Tensor total_len, torch::Tensor
   TORCH_CHECK(tokens.device() == history.device() && tokens.is_contiguous() &&
                   tokens.scalar_type() == torch::kInt64 && tokens.numel() == rows.numel(),
               "append_tokens: tokens (N) int64");
-  TORCH_CHECK(rows.numel() <= 65536, "append_tokens: at most 65536 rows");
+  TORCH_CHECK(rows.numel() <= 16384, "append_tokens: at most 16384 rows");
   if (rows.numel() == 0) return;
   const c10::DeviceGuard guard(history.device());
   append_tokens_kernel<<<dim3(1), dim3(256), 0, at::hip::getCurrentHIPStream()>>>(

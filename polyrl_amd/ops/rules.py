@@ -135,12 +135,15 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, rows: torch.Tensor,
         u = l / repetition where l > 0, else l * repetition, of tokens seen before
         u - frequency * (times in the output) - presence * (in the output) + bias
 
-    and -inf for what is not allowed, in 32 bits, rounded once.  ``out``: where they go,
-    ``out=logits`` in place."""
+    and -inf for what is not allowed, in 32 bits, rounded once (no autograd).  ``out``: where
+    they go, ``out=logits`` in place, else apart from it."""
     if logits.dim() != 2 or logits.shape[1] != rules.vocab:
         raise ValueError(f"adjust_logits: logits (N, {rules.vocab})")
     if rows.dtype != torch.int32 or rows.shape != logits.shape[:1]:
         raise ValueError("adjust_logits: rows (N,) int32")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("adjust_logits has no gradients: call it under "
+                           "torch.no_grad()")
     if logits.is_cuda:
         ext = _ops._require_ext()
         if out is None:

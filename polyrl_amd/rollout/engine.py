@@ -148,6 +148,8 @@ class Request:
     # prefix sharing: a group parent prefills once for n samples; children
     # are forked at first-token sampling (radix-cache capability)
     group_children: Optional[List[str]] = None
+    # what the first token may be (words of ops.token_words), None for all
+    first_words: Optional[np.ndarray] = None
 
     @property
     def seq_len(self) -> int:
@@ -639,13 +641,14 @@ class Engine:
             if r.sampling.adapter == name:
                 raise RuntimeError(f"adapter {name!r} is in use by {r.rid}")
 
-    def check_sampling(self, sampling: SamplingParams, input_ids: List[int]):
-        """ValueError for an adapter that is not loaded or rules that cannot hold
-        (:meth:`add_request` calls it)."""
+    def _check_sampling(self, sampling: SamplingParams, input_ids: List[int]):
+        """ValueError for an adapter that is not loaded or rules that cannot hold;
+        what the first token may be."""
         if sampling.adapter and sampling.adapter not in self.adapters:
             raise ValueError(f"no adapter {sampling.adapter!r}")
-        if sampling.has_rules:
-            self.rules.check(sampling, len(input_ids))
+        if not sampling.has_rules:
+            return None
+        return self.rules.check(sampling, len(input_ids))
 
     def _adapter_slots(self, reqs: List[Request]) -> Optional[List[int]]:
         """Adapter slots of requests, None if none has one."""
@@ -656,9 +659,9 @@ class Engine:
     def add_request(self, rid: str, input_ids: List[int],
                     sampling: SamplingParams):
         assert len(input_ids) > 0
-        self.check_sampling(sampling, input_ids)
+        words = self._check_sampling(sampling, input_ids)
         req = Request(rid=rid, input_ids=list(input_ids), sampling=sampling,
-                      arrival_t=time.time())
+                      arrival_t=time.time(), first_words=words)
         self.waiting.append(req)
         return rid
 
@@ -672,13 +675,14 @@ class Engine:
         copied per child so decode writes never touch shared pages).
         Child rids are '<prefix>-s0' .. '<prefix>-s<n-1>'."""
         assert n >= 1
-        self.check_sampling(sampling, input_ids)
+        words = self._check_sampling(sampling, input_ids)
         if n == 1 or not self.enable_prefix_sharing:
             for s_ in range(n):
                 self.add_request(f"{rid_prefix}-s{s_}", input_ids, sampling)
             return
         parent = Request(rid=f"{rid_prefix}-s0", input_ids=list(input_ids),
-                         sampling=sampling, arrival_t=time.time())
+                         sampling=sampling, arrival_t=time.time(),
+                         first_words=words)
         parent.group_children = [f"{rid_prefix}-s{s_}" for s_ in range(1, n)]
         self.waiting.append(parent)
 
@@ -991,10 +995,16 @@ class Engine:
         return tokens, lps
 
     def _next_mask(self, r: Request):
-        if r.sampling.token_mask is not None and not r.finished \
-                and not self.rules.advance(r):
+        if r.sampling.token_mask is None or r.finished:
+            return
+        try:
+            if not self.rules.advance(r):
+                r.finished = True
+                r.finish_reason = "stop"
+        except Exception as e:           # the caller's function: its request ends
+            print(f"[engine] token_mask of {r.rid}: {e!r}", flush=True)
             r.finished = True
-            r.finish_reason = "stop"
+            r.finish_reason = "abort"
 
     # ----------------------------------------------------- hybrid decoders
     def _hybrid_batch(self, items):
@@ -1298,7 +1308,8 @@ class Engine:
         Lp = len(parent.input_ids)
         children = [Request(rid=crid, input_ids=parent.input_ids,
                             sampling=parent.sampling, prefill_pos=Lp,
-                            arrival_t=parent.arrival_t)
+                            arrival_t=parent.arrival_t,
+                            first_words=parent.first_words)
                     for crid in child_rids]
         child_sids = []
         for c in children:

@@ -50,8 +50,9 @@ class RequestRules:
         self._slots: Dict[str, int] = {}
         self._free: List[int] = []
 
-    def check(self, sp, prompt_len: int) -> None:
-        """ValueError for rules that no table could hold."""
+    def check(self, sp, prompt_len: int) -> Optional[np.ndarray]:
+        """What the first token may be (:func:`allowed_words`); ValueError for rules that no
+        table could hold."""
         for name in ("repetition_penalty", "frequency_penalty",
                      "presence_penalty"):
             v = getattr(sp, name)
@@ -69,6 +70,7 @@ class RequestRules:
         words = allowed_words(sp, [], self.vocab)
         if not leaves_a_token(words, sp, self.vocab):
             raise ValueError("rules that leave no token")
+        return words
 
     def rows(self, reqs) -> Optional[torch.Tensor]:
         """Slots of the requests on the device, -1 where one has no rules; None if none
@@ -106,7 +108,7 @@ class RequestRules:
                        repetition=sp.repetition_penalty,
                        frequency=sp.frequency_penalty,
                        presence=sp.presence_penalty, bias=bias,
-                       allowed=allowed_words(sp, r.output_ids, self.vocab))
+                       allowed=r.first_words)
         self._free.pop()
         self._slots[r.rid] = slot
         return slot

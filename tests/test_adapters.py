@@ -272,7 +272,19 @@ def test_refusals(dev):
     with pytest.raises(error):                              # other adapters
         ops.adapter_add(y, x, a[:1].contiguous(), b[:1].contiguous(), scale[:1],
                         plan)
+    with pytest.raises(error):                              # rows on top of each other
+        ops.adapter_add(y, x, a, b, scale, plan,
+                        out=y[:1].expand(6, 16) if dev == "cuda" else y[:5])
     if dev == "cuda":
+        # a plan of fewer rows whose table is as long
+        many = ops.adapter_plan(torch.zeros(224, dtype=torch.int32, device=dev), 2)
+        big = [t.new_zeros(264, t.shape[1]) for t in (y, x)]
+        assert many.table.numel() == ops.adapter_plan(
+            torch.zeros(264, dtype=torch.int32, device=dev), 2).table.numel()
+        with pytest.raises(error):
+            ops.adapter_add(*big, a, b, scale, many)
+        with pytest.raises(error):
+            ops.adapter_add(y, x, a, b, scale, ops.adapter_plan(index.cpu(), 2))
         for bad in (x.float(), x.half()):
             with pytest.raises(error):
                 ops.adapter_add(y, bad, a, b, scale, plan)

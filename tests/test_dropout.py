@@ -138,7 +138,7 @@ def test_more_elements_than_31_bits():
 
 @pytest.mark.gpu
 def test_captured():
-    """Forward and backward in a graph, a seed that moves on, an eager graph beside it."""
+    """Forward and backward in a graph whose seed moves on."""
     g = torch.Generator().manual_seed(3)
     x = torch.randn(64, 100, generator=g).cuda().requires_grad_()
     seed = torch.tensor([100], device="cuda")

@@ -274,6 +274,11 @@ def test_refusals(dev):
     with pytest.raises(error):
         ops.adjust_logits(logits, rules, rows.long())
     with pytest.raises(error):
+        ops.adjust_logits(logits.clone().requires_grad_(), rules, rows)
+    with pytest.raises(error):                    # rows on top of each other
+        ops.adjust_logits(logits, rules, rows, out=logits[0].expand(3, 40)
+                          if dev == "cuda" else logits[:2])
+    with pytest.raises(error):
         ops.append_tokens(rules, rows, torch.zeros(2, dtype=torch.int64, device=dev))
     with pytest.raises(error):
         ops.append_tokens(rules, rows, torch.zeros(3, device=dev))

@@ -261,6 +261,11 @@ def test_grammar(models):
         engine(models[0][1]), [(list(range(40)), greedy(9))])[0].output_ids
     with pytest.raises(ValueError):               # nothing from the start
         e.add_request("x", [1], greedy(3, token_mask=lambda out: []))
+    # a function that fails ends its own request
+    d, f = run(e, [(PROMPTS[0], greedy(5, token_mask=lambda out: [9, 8][:2 // (2 - len(out))])),
+                   (PROMPTS[1], greedy(9))])
+    assert len(d.output_ids) == 2 and d.finish_reason == "abort"
+    assert f.output_ids == b.output_ids
 
 
 def test_more_requests_than_slots(models):
