@@ -79,9 +79,10 @@ DEV_INLINE i32x4_t load_some(const T* p, int have) {
 }
 
 // ---------------------------------------------------------------------- plan
-// plan: tiles, then (4 ints each) adapter, first place, rows; then the rows by place.
-// Rows without an adapter come last, as tiles of adapter -1.
-constexpr int XCDS = 8;               // dies, each with an L2 of its own
+// plan: the number of tiles; for each one (4 ints) its adapter and number of rows; for
+// each one its rows, in places for a whole tile, so that a block knows where to read
+// them before it knows anything else.  Rows without an adapter come last, as tiles of
+// adapter -1.
 constexpr int PLAN_HEAD = 4;
 constexpr int MOST_SLOTS = 4095, MOST_RANK = 256;
 
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
                                                             int T, int slots, int tile,
                                                             int most) {
   __shared__ int count[MOST_SLOTS + 1], cursor[MOST_SLOTS + 1];
-  __shared__ int sum_rows[16], sum_tiles[16];
+  __shared__ int sums[16];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   for (int s = tid; s <= slots; s += 1024) count[s] = 0;
   __syncthreads();
@@ -140,25 +141,22 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
     if (__ffsll(lanes) - 1 == lane) atomicAdd(&count[s], __popcll(lanes));
   });
   __syncthreads();
-  // each thread a stretch of adapters, then sums of the threads before
+  // each thread a stretch of adapters, then the tiles of the threads before
   const int per = (slots + 1 + 1023) / 1024;
-  int rows = 0, tiles = 0;
-  for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
-    rows += count[s];
+  int tiles = 0;
+  for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s)
     tiles += (count[s] + tile - 1) / tile;
-  }
-  int at = wave_scan(rows), n = wave_scan(tiles);
-  if (lane == 63) sum_rows[wid] = at, sum_tiles[wid] = n;
+  int n = wave_scan(tiles);
+  if (lane == 63) sums[wid] = n;
   __syncthreads();
-  for (int w = 0; w < wid; ++w) at += sum_rows[w], n += sum_tiles[w];
+  for (int w = 0; w < wid; ++w) n += sums[w];
   if (tid == 1023) plan[0] = n;
-  at -= rows, n -= tiles;
+  n -= tiles;
   i32x4_t* entry = reinterpret_cast<i32x4_t*>(plan + PLAN_HEAD);
   for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
-    cursor[s] = at;
+    cursor[s] = n * tile;
     for (int i = 0; i < count[s]; i += tile, ++n)
-      entry[n] = i32x4_t{s < slots ? s : -1, at + i, min(tile, count[s] - i), 0};
-    at += count[s];
+      entry[n] = i32x4_t{s < slots ? s : -1, min(tile, count[s] - i), 0, 0};
   }
   __syncthreads();
   int* order = plan + PLAN_HEAD + 4 * most;
@@ -175,7 +173,8 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
 struct Shape {
   int T, K, N, parts, rank, rank16;   // rank16: rank rounded up to whole tiles of 16
   long ldx, ldy, ldo;
-  int split, most;
+  int split, most;                    // shares of the inner dimension; places for tiles
+  int places;                         // most times the rows of a tile
   int first[9];                       // columns of the parts
 };
 
@@ -225,26 +224,25 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
   const int groups = (z.rank16 / 16 * z.parts + CT - 1) / CT;
-  // A die takes a stretch of the tiles, which lie in the order of their adapters: few
-  // adapters' matrices for each L2.  Reads wait for each other in three steps: the tile;
-  // its rows and the adapter's rank; what they name.
-  const int n = plan[0] * subs, stretch = (n + XCDS - 1) / XCDS;
-  int id = blockIdx.x / XCDS;
+  int id = blockIdx.x;
   const int share = id % z.split;
   id /= z.split;
-  const int group = id % groups;
-  id /= groups;
-  const int at = blockIdx.x % XCDS * stretch + id;
-  if (id >= stretch || at >= n) return;
-  const int tile = at / subs, sub = at % subs;
-  const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[tile];
-  const int slot = t[0], place = t[1] + sub * RT * 16, rows = t[2] - sub * RT * 16;
-  if (slot < 0 || rows <= 0) return;
-  const int rank = ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
+  const int group = id % groups, at = id / groups, tile = at / subs;
+  // Two steps of reads that wait for each other: the tile and its rows; what they name.
+  // (Rows past the tile and ranks past the adapter's are any, dropped below.)
+  const int place = at * RT * 16;
   const int* order = plan + PLAN_HEAD + 4 * z.most + place;
-  // rows of load j, and where this lane starts in them; rows past the tile and ranks
-  // past the adapter's are any, dropped below
   const int first = lane / 4 % 4 * 4, part_of = (lhi * 4 + lane % 4) * O::PER;
+  int row[RT][4];                     // rows of load j
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) row[r][j] = order[r * 16 + first + j];
+  const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[tile];
+  const int slot = t[0], rows = t[1] - at % subs * RT * 16;
+  if (tile >= plan[0] || slot < 0 || rows <= 0) return;
+  const int rank = ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
+  const int some = __builtin_amdgcn_readfirstlane(row[0][0]);
   const T* xr[RT][4];
   const T* base[CT];
   uint32_t ar[CT][4];                 // (a matrix is less than 2^30 bytes)
@@ -252,7 +250,7 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      xr[r][j] = x + (long)order[min(r * 16 + first + j, rows - 1)] * z.ldx + part_of;
+      xr[r][j] = x + (long)(r * 16 + first + j < rows ? row[r][j] : some) * z.ldx + part_of;
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     const int i = group * CT + c;
@@ -310,12 +308,13 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
   __syncthreads();
   for (int o = threadIdx.x; o < RT * CT * 256; o += NW * 64) {
     const int i = group * CT + o / 256 % CT, r = o / 256 / CT;
-    const int row = r * 16 + o % 256 / 16, j = i / z.parts * 16 + o % 16;
-    if (row >= rows || j >= rank) continue;
+    const int j = i / z.parts * 16 + o % 16;
+    if (r * 16 + o % 256 / 16 >= rows || j >= rank) continue;
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += red[w * RT * CT * 256 + o];
-    h[(((long)share * z.T + place + row) * z.parts + i % z.parts) * z.rank16 + j] = v;
+    h[(((long)share * z.places + place + r * 16 + o % 256 / 16) * z.parts + i % z.parts) *
+          z.rank16 + j] = v;
   }
 }
 
@@ -383,15 +382,18 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
   const Place at(z, cols, FEW_COLS);
-  if (at.tile >= plan[0]) return;
+  const int place = at.tile * 16;
+  const int own = (plan + PLAN_HEAD + 4 * z.most + place)[l15];
   const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[at.tile];
-  const int slot = t[0], place = t[1], rows = t[2];
-  if (slot < 0 && out == y) return;
+  const int slot = t[0], rows = t[1];
+  if (at.tile >= plan[0] || (slot < 0 && out == y)) return;
   const int rank = slot < 0 ? 0 : ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
   const int n0 = at.n0 + wid * 64, end = at.end;
   const bool whole = OUT_WORDS && n0 + 64 <= end;
   // all that is read is on its way before any of it is waited for
-  const long row = (plan + PLAN_HEAD + 4 * z.most + place)[min(l15, rows - 1)];
+  // (by all lanes: inside the choice it would be the first lane past the tile's)
+  const int some = __builtin_amdgcn_readfirstlane(own);
+  const long row = l15 < rows ? own : some;
   const T* bb = b + (long)max(slot, 0) * z.N * z.rank;
   i32x4_t bv[S][4];
   auto load_b = [&](int j0) {
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     if (r < rows && j0 + j < rank)
       v = shares_sum(h + (((long)place + r) * z.parts + at.part) * z.rank16 + j0 + j,
-                     (long)z.T * z.parts * z.rank16, z.split);
+                     (long)z.places * z.parts * z.rank16, z.split);
     const Four<T> f(v, s, rank - j0 - j);
     f.put(&hs[0][r][j], f.hi);
     if (SPLIT) f.put(&hs[SPLIT ? 1 : 0][r][j], f.lo);
@@ -487,23 +489,24 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
   const Place at(z, cols, COLS);
-  if (at.tile >= plan[0]) return;
+  const int place = at.tile * 64, mine = wid * 16 + lhi * 4;   // this lane's first row
+  const i32x4_t own = *reinterpret_cast<const i32x4_t*>(
+      plan + PLAN_HEAD + 4 * z.most + place + mine);
+  const int some = (plan + PLAN_HEAD + 4 * z.most)[place];
   const i32x4_t t = reinterpret_cast<const i32x4_t*>(plan + PLAN_HEAD)[at.tile];
-  const int slot = t[0], place = t[1], rows = t[2];
-  if (slot < 0 && out == y) return;
+  const int slot = t[0], rows = t[1];
+  if (at.tile >= plan[0] || (slot < 0 && out == y)) return;
   const int rank = slot < 0 ? 0 : ranks ? min(max(ranks[slot], 0), z.rank) : z.rank;
-  const int* order = plan + PLAN_HEAD + 4 * z.most + place;
   const int n0 = at.n0, end = at.end;
   const float s = slot < 0 ? 0.f : scale[slot];
-  const int mine = wid * 16 + lhi * 4;            // this lane's first row
   const bool whole = OUT_WORDS && n0 + COLS <= end;
   int row[4];
   Word yv[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) row[i] = order[min(mine + i, rows - 1)];
+  for (int i = 0; i < 4; ++i) row[i] = mine + i < rows ? own[i] : some;
   constexpr int NB = COLS * GRAN / 256;           // words of b that a thread brings
   constexpr int NH = 64 * PRE / 4 / 256;
-  const long share = (long)z.T * z.parts * z.rank16;
+  const long share = (long)z.places * z.parts * z.rank16;
   const T* bb = b + ((long)max(slot, 0) * z.N + n0) * z.rank;
   const float* hh = h + ((long)place * z.parts + at.part) * z.rank16;
   i32x4_t bv[NB];
@@ -609,7 +612,7 @@ torch::Tensor adapter_plan(torch::Tensor index, int64_t slots) {
               " adapters");
   const c10::DeviceGuard guard(index.device());
   const long T = index.numel(), most = most_tiles(T, slots);
-  auto plan = torch::empty({PLAN_HEAD + 4 * most + T}, index.options());
+  auto plan = torch::empty({PLAN_HEAD + (4 + tile_rows(T)) * most}, index.options());
   if (T == 0) return plan;
   adapter_plan_kernel<<<dim3(1), dim3(1024), 0, at::hip::getCurrentHIPStream()>>>(
       plan.data_ptr<int>(), index.data_ptr<int>(), (int)T, (int)slots, tile_rows(T),
@@ -639,14 +642,13 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
   // where it has twice as many and reads x for each group
   const int tiles = z.rank16 / 16 * z.parts, most_ct = RT == 1 ? 2 : 4;
   const int groups = (tiles + most_ct - 1) / most_ct, CT = (tiles + groups - 1) / groups;
-  const long blocks = ((long)z.most * subs + XCDS - 1) / XCDS * XCDS *
-                      ((tiles + CT - 1) / CT);
+  const long blocks = (long)z.most * subs * ((tiles + CT - 1) / CT);
   // shares of the inner dimension until there are 512 blocks, each wave with a round at
   // least; no more than up to four, because up adds them in every block
   z.split = (int)std::max<long>(
       1, std::min<long>({512 / blocks, (long)z.K * y.element_size() / (NW * 256),
                          MOST_SPLIT}));
-  auto h = torch::empty({(long)z.split * z.T * z.parts * z.rank16},
+  auto h = torch::empty({(long)z.split * z.places * z.parts * z.rank16},
                         y.options().dtype(torch::kFloat32));
   TORCH_CHECK(blocks * z.split < (1L << 31), "adapter_add: too many rows");
   auto down = [&](auto kern, int waves) {
@@ -728,8 +730,9 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
   z.rank = (int)r, z.rank16 = (int)((r + 15) / 16 * 16);
   z.ldx = x.stride(0), z.ldy = y.stride(0), z.ldo = out.stride(0);
   z.most = (int)most_tiles(T, S);
+  z.places = z.most * tile_rows(T);
   TORCH_CHECK(plan.device() == y.device() && plan.scalar_type() == torch::kInt32 &&
-                  rows == T && plan.numel() == PLAN_HEAD + 4L * z.most + T,
+                  rows == T && plan.numel() == PLAN_HEAD + (4L + tile_rows(T)) * z.most,
               "adapter_add: a plan of other rows");
   const long size = y.element_size();
   auto whole = [&](const torch::Tensor& t, long row) {

@@ -278,9 +278,9 @@ def test_refusals(dev):
     if dev == "cuda":
         # a plan of fewer rows whose table is as long
         many = ops.adapter_plan(torch.zeros(224, dtype=torch.int32, device=dev), 2)
-        big = [t.new_zeros(264, t.shape[1]) for t in (y, x)]
+        big = [t.new_zeros(230, t.shape[1]) for t in (y, x)]
         assert many.table.numel() == ops.adapter_plan(
-            torch.zeros(264, dtype=torch.int32, device=dev), 2).table.numel()
+            torch.zeros(230, dtype=torch.int32, device=dev), 2).table.numel()
         with pytest.raises(error):
             ops.adapter_add(*big, a, b, scale, many)
         with pytest.raises(error):
