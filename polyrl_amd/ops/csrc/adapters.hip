@@ -14,9 +14,10 @@
 // read A in every block of columns; h is 1% of y.)
 //
 // What bounds it: memory, prompts by y and out (6504 rows, ranks 32, the four projections of
-// 4096 / 6144 / 14336 numbers, 1.43 GB: 363 us, 3.9 TB/s; the widest, 746 MB, 153 us, where a
+// 4096 / 6144 / 14336 numbers, 1.43 GB: 370 us, 3.9 TB/s; the widest, 746 MB, 152 us, where a
 // copy of the same tiles takes 131), decode by the adapters (57 rows of as many adapters of
-// ranks 64 and 32, 0.45 GB: 152 us, 2.9 TB/s); one row by nine launches, 41 us (34 in a graph).
+// ranks 64 and 32, 0.45 GB: 148 us, 3.0 TB/s); one row by nine launches, 34 us in a graph and
+// 43 issued one by one.
 //
 // Matrix cores: 16x16x32 in bf16, 16x16x4 in fp32.  h is a sum in 32 bits; as an operand
 // in bf16 it is split in two bf16 numbers, h = hi + lo, each with its own product, so that what
