@@ -30,6 +30,12 @@ def token_words(tokens, vocab: int) -> np.ndarray:
     return np.packbits(bits, bitorder="little").view(np.int32)
 
 
+def in_32_bits(v: float) -> float:
+    """v as the kernels see it: what fp32 does not hold is infinite or 0."""
+    with np.errstate(over="ignore", under="ignore"):
+        return float(np.float32(v))
+
+
 class LogitRules:
     """Rules of ``slots`` requests over a vocabulary: tensors by slot, which a program
     may also write itself.
@@ -77,6 +83,7 @@ class LogitRules:
         self._check(slot)
         for name, v in (("repetition", repetition), ("frequency", frequency),
                         ("presence", presence)):
+            v = in_32_bits(v)
             if not math.isfinite(v) or name == "repetition" and v <= 0:
                 raise ValueError(f"LogitRules: {name} {v}")
         words = np.asarray([*prompt, *output], dtype=np.int32)
@@ -102,7 +109,7 @@ class LogitRules:
             tokens = np.full(self.biases, -1, np.int32)
             values = np.zeros(self.biases, np.float32)
             for i, (t, v) in enumerate(pairs):
-                tokens[i], values[i] = int(t), v
+                tokens[i], values[i] = int(t), in_32_bits(v)
             dev = self.history.device
             self.bias_tokens[slot] = torch.from_numpy(tokens).to(dev)
             self.bias_values[slot] = torch.from_numpy(values).to(dev)

@@ -9,7 +9,7 @@ import numpy as np
 import torch
 
 import polyrl_amd.ops as ops
-from ..ops.rules import MOST_BIASES, MOST_TOKENS, token_words
+from ..ops.rules import MOST_BIASES, MOST_TOKENS, in_32_bits, token_words
 
 
 def allowed_words(sp, output_ids, vocab: int) -> Optional[np.ndarray]:
@@ -30,7 +30,8 @@ def allowed_words(sp, output_ids, vocab: int) -> Optional[np.ndarray]:
 
 def leaves_a_token(words: Optional[np.ndarray], sp, vocab: int) -> bool:
     """Whether some token is allowed that no bias of -inf bans."""
-    banned = [int(t) for t, v in dict(sp.logit_bias).items() if v == -math.inf]
+    banned = [int(t) for t, v in dict(sp.logit_bias).items()
+              if in_32_bits(v) == -math.inf]
     if words is None:
         return len(banned) < vocab
     bits = np.unpackbits(words.view(np.uint8), bitorder="little")[:vocab]
@@ -55,14 +56,15 @@ class RequestRules:
         table could hold."""
         for name in ("repetition_penalty", "frequency_penalty",
                      "presence_penalty"):
-            v = getattr(sp, name)
+            v = in_32_bits(getattr(sp, name))
             if not math.isfinite(v) or name[0] == "r" and v <= 0:
                 raise ValueError(f"{name} {v}")
         bias = dict(sp.logit_bias)
         if len(bias) > MOST_BIASES:
             raise ValueError(f"more than {MOST_BIASES} biases")
         for t, v in bias.items():
-            if not 0 <= int(t) < self.vocab or math.isnan(v) or v == math.inf:
+            if not 0 <= int(t) < self.vocab or math.isnan(v) \
+                    or in_32_bits(v) == math.inf:
                 raise ValueError(f"logit_bias {v} of token {t}")
         if prompt_len > self.capacity:
             raise ValueError(f"rules for a prompt of {prompt_len} tokens, more "

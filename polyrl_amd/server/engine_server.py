@@ -64,8 +64,12 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
     async def generate(request: Request):
         body = await request.json()
         input_ids: List[int] = body["input_ids"]
-        sp = _sp(body.get("sampling_params", {}))
-        n = int(body.get("sampling_params", {}).get("n", 1))
+        try:
+            sp = _sp(body.get("sampling_params", {}))
+            n = int(body.get("sampling_params", {}).get("n", 1))
+        except (ValueError, TypeError, AttributeError) as e:
+            return JSONResponse({"success": False,
+                                 "message": f"sampling_params: {e}"}, 400)
         want_lp = bool(body.get("return_logprob", False))
         stream = bool(body.get("stream", False))
 
@@ -138,21 +142,24 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
             return JSONResponse({"success": False,
                                  "message": "sender not in allowed CIDRs"},
                                 403)
+        from safetensors import SafetensorError
         from safetensors.torch import load, load_file
         if request.headers.get("content-type", "").startswith(
                 "application/json"):
             body = await request.json()
-            name, scaling = str(body["name"]), float(body.get("scaling", 1.0))
+            name, scaling = body.get("name"), body.get("scaling", 1.0)
             read = lambda: load_file(body["path"])
         else:
             raw = await request.body()
-            name = request.headers.get("x-adapter-name", "")
-            scaling = float(request.headers.get("x-adapter-scaling", "1.0"))
+            name = request.headers.get("x-adapter-name")
+            scaling = request.headers.get("x-adapter-scaling", "1.0")
             read = lambda: load(raw)
         try:
+            name, scaling = str(name or ""), float(scaling)
             await asyncio.get_running_loop().run_in_executor(
                 None, lambda: runner.load_adapter(name, read(), scaling))
-        except (ValueError, RuntimeError, OSError) as e:
+        except (ValueError, TypeError, KeyError, RuntimeError, OSError,
+                SafetensorError) as e:
             return JSONResponse({"success": False, "message": str(e)}, 400)
         return {"success": True, "adapters": engine.adapters}
 
@@ -165,7 +172,7 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
         body = await request.json()
         try:
             await asyncio.get_running_loop().run_in_executor(
-                None, lambda: runner.unload_adapter(str(body["name"])))
+                None, lambda: runner.unload_adapter(str(body.get("name"))))
         except (ValueError, RuntimeError) as e:
             return JSONResponse({"success": False, "message": str(e)}, 400)
         return {"success": True, "adapters": engine.adapters}

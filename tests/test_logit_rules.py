@@ -1,5 +1,6 @@
 """Penalties, biases and allowed tokens on logits, against 64 bits."""
 import math
+import warnings
 
 import numpy as np
 import pytest
@@ -291,3 +292,17 @@ def test_refusals(dev):
             ops.adjust_logits(logits, rules, rows.cpu())
         with pytest.raises(error):
             ops.adjust_logits(torch.zeros(40, 3, device=dev).t(), rules, rows)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_numbers_that_32_bits_do_not_hold(dev):
+    """A rule is what its 32 bits say: a repetition of 1e-60 would be a division by 0."""
+    rules = ops.LogitRules(1, 40, 6, dev, biases=2)
+    for kw in (dict(repetition=1e-60), dict(repetition=1e60),
+               dict(frequency=-1e60), dict(presence=1e60)):
+        with pytest.raises(ValueError):
+            rules.set(0, **kw)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        rules.set(0, bias={1: -1e60, 2: 5.0})
+    assert rules.bias_values[0].tolist() == [-math.inf, 5.0]

@@ -302,6 +302,22 @@ def test_rules_that_cannot_hold(models):
     assert not e.has_work()
 
 
+def test_rules_that_32_bits_do_not_hold(models):
+    """1e60 is infinite to the kernels: refused like infinities, and a ban below."""
+    e = engine(models[0][1])
+    v = e.cfg.vocab_size
+    for kw in (dict(repetition_penalty=1e-60), dict(repetition_penalty=1e60),
+               dict(frequency_penalty=1e60), dict(presence_penalty=-1e60),
+               dict(logit_bias={3: 1e60}), dict(logit_bias={t: -1e60 for t in range(v)}),
+               dict(logit_bias={3: -1e60}, allowed_token_ids=(3,))):
+        with pytest.raises(ValueError):
+            e.add_request("r", PROMPTS[0], greedy(4, **kw))
+    assert not e.has_work()
+    out, = run(e, [(PROMPTS[0], greedy(4, logit_bias={3: -1e60},
+                                       allowed_token_ids=(3, 5)))])
+    assert out.output_ids == [5] * 4
+
+
 def test_rules_on_hybrid_decoders():
     e = Engine(get_model_config("kuforax-debug"), device="cpu", dtype=torch.float32,
                kv_token_capacity=512, max_running_requests=4)
@@ -556,3 +572,39 @@ def test_prompt_steps_against_merged_weights(tiny, lens):
         if a:
             moved.append(float((lp[a] - lp[""]).abs().mean()))
     assert min(moved) > 0.2
+
+
+def test_http_requests_that_say_nothing(models, tmp_path):
+    """Fields of other types and files that are none are the caller's: 400."""
+    httpx = pytest.importorskip("httpx")
+    from polyrl_amd.rollout.runner import EngineRunner
+    from polyrl_amd.server.engine_server import create_app
+    e = engine(models[0][1])
+    runner = EngineRunner(e)
+    app = create_app(e, runner)
+    (tmp_path / "none").write_bytes(b"no tensors")
+
+    async def go():
+        async with httpx.AsyncClient(transport=httpx.ASGITransport(app=app),
+                                     base_url="http://t") as c:
+            for sp in (dict(logit_bias={"a": 1.0}), dict(logit_bias=[1, 2]),
+                       dict(repetition_penalty="high"), dict(frequency_penalty=None),
+                       dict(allowed_token_ids=5), dict(allowed_token_ids=["x"])):
+                r = await c.post("/generate", json={
+                    "input_ids": PROMPTS[0], "sampling_params": sp})
+                assert r.status_code == 400, sp
+            for body in (dict(name="a", path=str(tmp_path / "none")),
+                         dict(path=str(tmp_path / "none")), dict(name="a"),
+                         dict(name="a", path=str(tmp_path / "none"), scaling="x")):
+                r = await c.post("/load_adapter", json=body)
+                assert r.status_code == 400, body
+            r = await c.post("/load_adapter", content=b"no tensors",
+                             headers={"x-adapter-name": "a"})
+            assert r.status_code == 400
+            r = await c.post("/load_adapter", content=b"", headers={
+                "x-adapter-name": "a", "x-adapter-scaling": "x"})
+            assert r.status_code == 400
+            r = await c.post("/unload_adapter", json={})
+            assert r.status_code == 400
+        assert not runner._futures and not e.adapters
+    asyncio.run(go())
