@@ -14,8 +14,11 @@ the trainer's FSDP parameters, so weight-version updates are plain copies
 """
 from __future__ import annotations
 
+import contextlib
+import gc
 import math
 import time
+import weakref
 from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional
 
@@ -89,6 +92,21 @@ def _gate_up(x: torch.Tensor, w: torch.Tensor, search: bool = True
 # at most ~16 captures over the whole 1..256 running-batch range
 DECODE_BUCKETS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128,
                   192, 256)
+
+
+@contextlib.contextmanager
+def _captured(graph, pool=None):
+    """``torch.cuda.graph`` without the garbage collector: a graph that it found then
+    (of an engine that was let go) would be destroyed while the stream captures, which
+    the runtime forbids, and an error in a destructor ends the process."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, pool=pool):
+            yield
+    finally:
+        if on:
+            gc.enable()
 
 
 def decode_bucket(b: int) -> int:
@@ -510,7 +528,9 @@ class Engine:
                                               tp_ctx=tp_ctx)
         else:
             self.model = InferenceModel(cfg, device, dtype, tp_ctx=tp_ctx)
-        self.model._engine_owner = self   # weight publishers flush the radix
+        # weight publishers flush the radix (weak: an engine that is let go goes at
+        # once, its graphs with it, and not when the cycle is found)
+        self.model._engine_owner = weakref.ref(self)
         self.tp = self.model.tp
         self.max_running = max_running_requests
         self.max_batched_tokens = max_num_batched_tokens
@@ -1143,7 +1163,7 @@ class Engine:
             for k, t in self.states.tensors.items():
                 t.copy_(saved[k])
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, pool=self._graph_pool):
+            with _captured(g, self._graph_pool):
                 st["res"] = self.model.forward_batch(sb, self.kv, self.states)
             if self._graph_pool is None:
                 self._graph_pool = g.pool()
@@ -1528,7 +1548,6 @@ class Engine:
                 st["ctx"] += 1
                 st["seed"] += 1
 
-            st["body"] = body
             # warmup on a side stream (kv writes land in slots that the
             # first real replay overwrites with identical data)
             side = torch.cuda.Stream()
@@ -1555,13 +1574,10 @@ class Engine:
                 if rule_rows is not None:   # (the warm-up's tokens are none)
                     st["rules"].total_len.copy_(lens)
             g = torch.cuda.CUDAGraph()
+            with _captured(g, self._graph_pool):
+                body()
             if self._graph_pool is None:
-                with torch.cuda.graph(g):
-                    body()
                 self._graph_pool = g.pool()
-            else:
-                with torch.cuda.graph(g, pool=self._graph_pool):
-                    body()
             st["graph"] = g
             self._graphs[key] = st
 

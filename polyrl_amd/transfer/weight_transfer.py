@@ -68,7 +68,8 @@ class WeightPublisher:
                     full = emb.full_tensor() if hasattr(emb, "full_tensor") else emb
                     c.update_named("lm_head.weight", full)
         for c in self.consumers:
-            eng = getattr(c, "_engine_owner", None)
+            owner = getattr(c, "_engine_owner", None)
+            eng = None if owner is None else owner()
             if eng is not None:
                 eng.flush_radix()   # cached KV prefixes are stale now
         if dist.is_available() and dist.is_initialized():

@@ -1,10 +1,13 @@
 """Requests of one batch with adapters and rules of their own, through the engine, its
 HTTP facade and from a trained adapter to a served one."""
 import asyncio
+import contextlib
+import gc
 import math
 import os
 import subprocess
 import sys
+import weakref
 
 import numpy as np
 import pytest
@@ -527,6 +530,63 @@ def test_captured_decode_is_the_eager_one(tiny, n):
             assert a.output_logprobs == b.output_logprobs
     allowed = [o for (p, sp), o in zip(jobs, got) if sp.allowed_token_ids]
     assert all(64 <= t < 512 for o in allowed for t in o.output_ids)
+
+
+@contextlib.contextmanager
+def no_collector():
+    gc.collect()
+    gc.disable()
+    try:
+        yield
+    finally:
+        gc.enable()
+
+
+@pytest.mark.parametrize("name", ["llama-debug-cpu", "kuforax-debug"])
+def test_engines_go_at_once(name):
+    """An engine that is let go goes with its last reference: its captured steps are not
+    left to a collector that may run while another engine captures."""
+    with no_collector():
+        e = Engine(get_model_config(name), device="cpu", dtype=torch.float32,
+                   kv_token_capacity=512, max_running_requests=4)
+        gone = [weakref.ref(t) for t in (e, e.model, e.kv)]
+        assert gone[1]()._engine_owner() is e
+        del e
+        assert [r() for r in gone] == [None] * 3
+
+
+@pytest.mark.parametrize("on", [True, False])
+def test_no_collection_while_a_step_is_captured(monkeypatch, on):
+    from polyrl_amd.rollout import engine as module
+
+    @contextlib.contextmanager
+    def graph(g, pool=None):
+        assert not gc.isenabled()
+        yield
+        assert not gc.isenabled()
+    monkeypatch.setattr(torch.cuda, "graph", graph)
+    try:
+        (gc.enable if on else gc.disable)()
+        with module._captured(None):
+            pass
+        assert gc.isenabled() == on
+        with pytest.raises(KeyError):
+            with module._captured(None, 1):
+                raise KeyError
+        assert gc.isenabled() == on
+    finally:
+        gc.enable()
+
+
+@pytest.mark.gpu
+def test_captured_steps_go_with_their_engine(tiny):
+    with no_collector():
+        e = gpu_engine(tiny, True)
+        run(e, mixed_jobs(4))
+        assert e._graphs
+        gone = [weakref.ref(e)] + [weakref.ref(t["tokens"]) for t in e._graphs.values()]
+        del e
+        assert not any(r() is not None for r in gone)
 
 
 @pytest.mark.gpu
