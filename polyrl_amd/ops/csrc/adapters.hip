@@ -20,8 +20,8 @@
 // 43 issued one by one.
 //
 // Matrix cores: 16x16x32 in bf16, 16x16x4 in fp32.  h is a sum in 32 bits; as an operand
-// in bf16 it is split in two bf16 numbers, h = hi + lo, each with its own product, so that what
-// is lost of it is 2^-16 and not the 2^-8 of one.
+// in bf16 it is cut into three bf16 numbers of 8 bits each, whose sum is h, each with its own
+// product, so that nothing is lost of it (two would lose 2^-16, one 2^-8).
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
@@ -320,25 +320,35 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
 }
 
 // ------------------------------------------------------------------------ up
-// h's numbers j .. j + 4 of a place, times s: the shares' sums in their order, split into hi
-// and lo; zeros from rank on
+// h's numbers j .. j + 4 of a place, times s (the shares' sums in their order, zeros from rank
+// on), as PARTS numbers of type T whose sum they are: of bf16 each the upper 8 bits of what
+// those before it leave, cut and not rounded, so that none is larger than h
+template <typename T> constexpr int PARTS = sizeof(T) == 2 ? 3 : 1;
+
 template <typename T>
 struct Four {
-  T hi[4], lo[4];
+  T part[PARTS<T>][4];
   DEV_INLINE Four(f32x4_t v, float s, int left) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float f = e < left ? v[e] * s : 0.f;
-      hi[e] = (T)f;
-      // (an infinite h has no lower part)
-      lo[e] = isfinite((float)hi[e]) ? (T)(f - (float)hi[e]) : (T)0.f;
+      float f = e < left ? v[e] * s : 0.f;
+      if (PARTS<T> == 1) {
+        part[0][e] = (T)f;
+        continue;
+      }
+#pragma unroll
+      for (int p = 0; p < PARTS<T>; ++p) {
+        const float cut = __uint_as_float(__float_as_uint(f) & 0xffff0000u);
+        part[p][e] = (T)cut;
+        f = isfinite(f) ? f - cut : 0.f;    // (an infinite h has no lower part)
+      }
     }
   }
-  DEV_INLINE static void put(T* at, const T (&v)[4]) {
+  DEV_INLINE void put(int p, T* at) const {
     struct alignas(sizeof(T) * 4) Word { T v[4]; };
     Word w;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w.v[e] = v[e];
+    for (int e = 0; e < 4; ++e) w.v[e] = part[p][e];
     *reinterpret_cast<Word*>(at) = w;
   }
 };
@@ -375,11 +385,10 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
     const float* __restrict__ scale, const int* __restrict__ ranks,
     const int* __restrict__ plan, const Shape z, int cols) {
   using O = Operand<T>;
-  constexpr bool SPLIT = sizeof(T) == 2;          // h as hi + lo
   constexpr int VEC = 16 / (int)sizeof(T), Q = 16 / VEC, PER_Q = VEC / 4;
   constexpr int PITCH = FEW_RANK + VEC, S = FEW_RANK / O::STEP;
   struct alignas(16) Word { T v[VEC]; };
-  __shared__ __attribute__((aligned(16))) T hs[SPLIT ? 2 : 1][16][PITCH];
+  __shared__ __attribute__((aligned(16))) T hs[PARTS<T>][16][PITCH];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
   const Place at(z, cols, FEW_COLS);
@@ -429,14 +438,14 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
       v = shares_sum(h + (((long)place + r) * z.parts + at.part) * z.rank16 + j0 + j,
                      (long)z.places * z.parts * z.rank16, z.split);
     const Four<T> f(v, s, rank - j0 - j);
-    f.put(&hs[0][r][j], f.hi);
-    if (SPLIT) f.put(&hs[SPLIT ? 1 : 0][r][j], f.lo);
+#pragma unroll
+    for (int p = 0; p < PARTS<T>; ++p) f.put(p, &hs[p][r][j]);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < S; ++k) {
       if (j0 + k * O::STEP >= rank) break;
 #pragma unroll
-      for (int p = 0; p < (SPLIT ? 2 : 1); ++p) {
+      for (int p = 0; p < PARTS<T>; ++p) {
         const i32x4_t hv =
             *reinterpret_cast<const i32x4_t*>(&hs[p][l15][k * O::STEP + lhi * O::PER]);
 #pragma unroll
@@ -482,11 +491,10 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
     const float* __restrict__ scale, const int* __restrict__ ranks,
     const int* __restrict__ plan, const Shape z, int cols) {
   using O = Operand<T>;
-  constexpr bool SPLIT = sizeof(T) == 2;          // h as hi + lo
   constexpr int VEC = 16 / (int)sizeof(T), COLS = 16 * VEC, PITCH = PRE + VEC;
   constexpr int GRAN = PRE / VEC;                 // 16-byte words of a row in LDS
   struct alignas(16) Word { T v[VEC]; };
-  __shared__ __attribute__((aligned(16))) T bs[COLS][PITCH], hs[SPLIT ? 2 : 1][64][PITCH];
+  __shared__ __attribute__((aligned(16))) T bs[COLS][PITCH], hs[PARTS<T>][64][PITCH];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int l15 = lane & 15, lhi = lane >> 4;
   const Place at(z, cols, COLS);
@@ -555,24 +563,24 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
     for (int i = 0; i < NH; ++i) {
       const int g = threadIdx.x + i * 256, r = g / (PRE / 4), j = g % (PRE / 4) * 4;
       const Four<T> f(hv[i], s, rank - j0 - j);
-      f.put(&hs[0][r][j], f.hi);
-      if (SPLIT) f.put(&hs[SPLIT ? 1 : 0][r][j], f.lo);
+#pragma unroll
+      for (int p = 0; p < PARTS<T>; ++p) f.put(p, &hs[p][r][j]);
     }
     __syncthreads();
     if (wid * 16 < rows)
 #pragma unroll
       for (int k = 0; k < PRE; k += O::STEP) {
         if (j0 + k >= rank) break;
-        i32x4_t hw[SPLIT ? 2 : 1];
+        i32x4_t hw[PARTS<T>];
 #pragma unroll
-        for (int p = 0; p < (SPLIT ? 2 : 1); ++p)
+        for (int p = 0; p < PARTS<T>; ++p)
           hw[p] = *reinterpret_cast<const i32x4_t*>(&hs[p][wid * 16 + l15][k + lhi * O::PER]);
 #pragma unroll
         for (int c = 0; c < VEC; ++c) {
           const i32x4_t bw =
               *reinterpret_cast<const i32x4_t*>(&bs[c * 16 + l15][k + lhi * O::PER]);
 #pragma unroll
-          for (int p = 0; p < (SPLIT ? 2 : 1); ++p) acc[c] = O::mul(hw[p], bw, acc[c]);
+          for (int p = 0; p < PARTS<T>; ++p) acc[c] = O::mul(hw[p], bw, acc[c]);
         }
       }
   }

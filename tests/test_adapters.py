@@ -209,6 +209,33 @@ def test_result_does_not_hang_on_the_order_of_rows():
         assert torch.equal(got, want[p])
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T,r", [(3, 4), (40, 70), (300, 4), (300, 70)])
+def test_inner_sums_keep_32_bits(dev, dtype, T, r):
+    """Whole numbers whose every sum is below 2^24: 32 bits hold them all, so that the
+    result is the exact one, rounded once.  y is the negative of the rounded product, which
+    leaves the places that 16 bits of h would lose."""
+    K, widths, S = 64, (40, 24), 2
+    g = torch.Generator().manual_seed(11)
+    x = torch.randint(128, 256, (T, K), generator=g).double()
+    a = torch.randint(128, 256, (S, len(widths), r, K), generator=g).double()
+    b = torch.zeros(S, sum(widths), r, dtype=torch.double)
+    at = torch.rand(b.shape, generator=g).topk(4, -1).indices
+    b.scatter_(2, at, 1.0)                       # 4 * 64 * 255 * 255 < 2^24
+    index = torch.arange(T, dtype=torch.int32) % S
+    h = torch.einsum("tprk,tk->tpr", a[index.long()], x)
+    h = h.repeat_interleave(torch.tensor(widths), 1)
+    total = (b[index.long()] * h).sum(-1)
+    assert total.max() < 1 << 24
+    y = -total.to(BF16).double()
+    want = (y + total).to(dtype)
+    y, x, a, b = (t.to(dtype).to(dev) for t in (y, x, a, b))
+    got = ops.adapter_add(y, x, a, b, torch.ones(S, device=dev),
+                          ops.adapter_plan(index.to(dev), S), widths)
+    assert torch.equal(got.cpu(), want)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [6, 400])
 def test_captured(T):
