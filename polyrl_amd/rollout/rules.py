@@ -72,7 +72,8 @@ class RequestRules:
         words = allowed_words(sp, [], self.vocab)
         if not leaves_a_token(words, sp, self.vocab):
             raise ValueError("rules that leave no token")
-        return words
+        # (kept until the first token is drawn: a mask may fill its words again)
+        return None if words is None else words.copy()
 
     def rows(self, reqs) -> Optional[torch.Tensor]:
         """Slots of the requests on the device, -1 where one has no rules; None if none

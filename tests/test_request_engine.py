@@ -271,6 +271,31 @@ def test_grammar(models):
     assert f.output_ids == b.output_ids
 
 
+def test_masks_of_one_buffer(models):
+    """A grammar that fills the same words again for every call: each request goes by what
+    the words were when it was asked."""
+    words = np.zeros(16, np.int32)
+
+    def mask(ids):
+        def f(out):
+            words[:] = 0
+            t = ids[len(out)]
+            words.view(np.uint32)[t // 32] = 1 << t % 32
+            return words
+        return f
+    ways = [[10, 11, 12], [100, 101, 102], [511, 31, 32]]
+    e = engine(models[0][1])
+    for o, ids in zip(run(e, [(PROMPTS[0], greedy(3, token_mask=mask(ids)))
+                              for ids in ways]), ways):
+        assert o.output_ids == ids
+    e.add_request_group("g", PROMPTS[0], greedy(3, token_mask=mask(ways[0])), 2)
+    e.add_request("x", PROMPTS[1], greedy(3, token_mask=mask(ways[1])))
+    outs = {}
+    while e.has_work():
+        outs.update((o.rid, o.output_ids) for o in e.step())
+    assert outs == {"g-s0": ways[0], "g-s1": ways[0], "x": ways[1]}
+
+
 def test_more_requests_than_slots(models):
     """Groups that fork past the running limit, and biases that outgrow the table."""
     e = engine(models[0][1], max_running_requests=2)
