@@ -16,6 +16,7 @@ from typing import Dict, Iterable, List, Tuple
 import torch
 
 import polyrl_amd.ops as ops
+from ..ops.rules import in_32_bits
 
 # parts of the fused projections, in the order of their rows
 PROJECTIONS = {"qkv": ("q", "k", "v"), "o": ("o",), "gate_up": ("gate", "up"),
@@ -45,6 +46,7 @@ class AdapterPool:
                        "down": (h,)}
         inner = {"qkv": h, "o": hq, "gate_up": h, "down": ff}
         wide = -(-rank // 8) * 8          # rows of B in whole 16-byte words
+        self.dtype = model.dtype
         new = dict(dtype=model.dtype, device=model.device)
         self.layers = [
             {proj: (torch.zeros(slots, len(w), wide, inner[proj], **new),
@@ -78,7 +80,7 @@ class AdapterPool:
         (out, r) of any of the seven projections, as ``models.lora.export_adapter`` and
         common adapter files name them.  A name that is there already is replaced."""
         parts = self._parts(state_dict)
-        if not name or not math.isfinite(scaling):
+        if not name or not math.isfinite(in_32_bits(scaling)):
             raise ValueError(f"adapter {name!r}: scaling {scaling}")
         slot = self.names.get(name)
         if slot is None:
@@ -86,6 +88,10 @@ class AdapterPool:
             if not free:
                 raise RuntimeError(f"all {self.slots} adapter slots are taken")
             slot = min(free)
+        # all that can be refused comes before the slot's first change: an adapter of this
+        # name stays whole
+        parts = {key: [t.to(device=self.scale.device, dtype=self.dtype) for t in pair]
+                 for key, pair in parts.items()}
         for layer in self.layers:
             for a, b in layer.values():
                 a[slot].zero_()

@@ -176,6 +176,30 @@ def test_adapters_that_do_not_fit(models):
 # ------------------------------------------------------------------- rules
 
 
+def test_refused_replacements_leave_what_was_there(models):
+    """A scaling that 32 bits do not hold, tensors that do not convert: the adapter of that name answers as before."""
+    e = serving(models)
+    job = [(PROMPTS[0], greedy(adapter="one"))]
+    want, = run(e, job)
+    sd, _ = export_adapter(models[1][0])
+    held = [t.clone() for layer in e.model.adapters.layers for p in layer.values()
+            for t in p]
+    for scaling in (1e39, -1e60, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            e.load_adapter("one", sd, scaling)
+    with pytest.raises(ValueError):               # of a new name: no slot is taken
+        e.load_adapter("three", sd, 1e39)
+    last = list(sd)[-1]
+    with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+        e.load_adapter("one", {**sd, last: sd[last].to("meta")}, 1.0)
+    assert e.adapters == ["one", "two"]
+    now = [t for layer in e.model.adapters.layers for p in layer.values() for t in p]
+    assert all(torch.equal(a, b) for a, b in zip(now, held))
+    got, = run(e, job)
+    assert got.output_ids == want.output_ids
+    assert got.output_logprobs == want.output_logprobs
+
+
 def rolled(models, prompt, sp, adapter=""):
     """Greedy tokens under rules and the model's own log-probabilities, token by token
     from the trainer's model."""
