@@ -22,7 +22,10 @@ MOST_BIASES = (1 << 12) - 1      # of a slot
 
 def token_words(tokens, vocab: int) -> np.ndarray:
     """Token ids as the bits of ceil(vocab / 32) int32 words."""
-    ids = np.asarray(list(tokens), dtype=np.int64)
+    try:
+        ids = np.asarray(list(tokens), dtype=np.int64)
+    except OverflowError:
+        raise ValueError("token ids outside of the vocabulary") from None
     if ids.size and (ids.min() < 0 or ids.max() >= vocab):
         raise ValueError("token ids outside of the vocabulary")
     bits = np.zeros((vocab + 31) // 32 * 32, dtype=np.uint8)
@@ -32,8 +35,11 @@ def token_words(tokens, vocab: int) -> np.ndarray:
 
 def in_32_bits(v: float) -> float:
     """v as the kernels see it: what fp32 does not hold is infinite or 0."""
-    with np.errstate(over="ignore", under="ignore"):
-        return float(np.float32(v))
+    try:
+        with np.errstate(over="ignore", under="ignore"):
+            return float(np.float32(v))
+    except OverflowError:                # a whole number beyond all floats
+        return math.inf if v > 0 else -math.inf
 
 
 class LogitRules:
@@ -94,7 +100,7 @@ class LogitRules:
         if len(pairs) > self.biases:
             raise ValueError(f"LogitRules: {len(pairs)} biases in {self.biases}")
         for t, v in pairs:
-            if not 0 <= int(t) < self.vocab or math.isnan(v):
+            if not 0 <= int(t) < self.vocab or math.isnan(in_32_bits(v)):
                 raise ValueError(f"LogitRules: bias {v} of token {t}")
         self.allow(slot, allowed)
         if len(words):
@@ -102,9 +108,9 @@ class LogitRules:
                 self.history.device)
         self.prompt_len[slot] = len(prompt)
         self.total_len[slot] = len(words)
-        self.repetition[slot] = repetition
-        self.frequency[slot] = frequency
-        self.presence[slot] = presence
+        self.repetition[slot] = in_32_bits(repetition)
+        self.frequency[slot] = in_32_bits(frequency)
+        self.presence[slot] = in_32_bits(presence)
         if self.biases:
             tokens = np.full(self.biases, -1, np.int32)
             values = np.zeros(self.biases, np.float32)

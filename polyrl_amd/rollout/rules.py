@@ -63,13 +63,18 @@ class RequestRules:
         if len(bias) > MOST_BIASES:
             raise ValueError(f"more than {MOST_BIASES} biases")
         for t, v in bias.items():
-            if not 0 <= int(t) < self.vocab or math.isnan(v) \
-                    or in_32_bits(v) == math.inf:
+            v = in_32_bits(v)
+            if not 0 <= int(t) < self.vocab or math.isnan(v) or v == math.inf:
                 raise ValueError(f"logit_bias {v} of token {t}")
         if prompt_len > self.capacity:
             raise ValueError(f"rules for a prompt of {prompt_len} tokens, more "
                              f"than {self.capacity}")
-        words = allowed_words(sp, [], self.vocab)
+        try:
+            words = allowed_words(sp, [], self.vocab)
+        except ValueError:
+            raise
+        except Exception as e:               # the caller's token_mask
+            raise ValueError(f"token_mask: {e!r}") from e
         if not leaves_a_token(words, sp, self.vocab):
             raise ValueError("rules that leave no token")
         # (kept until the first token is drawn: a mask may fill its words again)

@@ -370,6 +370,40 @@ def test_rules_that_32_bits_do_not_hold(models):
     assert out.output_ids == [5] * 4
 
 
+def test_numbers_that_no_table_holds(models):
+    """Token ids beyond 64 bits, numbers beyond floats, a mask that fails at once: the
+    request is refused as others are."""
+    from polyrl_amd.ops import LogitRules, token_words
+    e = engine(models[0][1])
+
+    def fails(out):
+        raise KeyError("state")
+    for kw in (dict(allowed_token_ids=(2 ** 70,)), dict(allowed_token_ids=(-2 ** 70, 3)),
+               dict(logit_bias={3: 10 ** 400}), dict(logit_bias={2 ** 70: 1.0}),
+               dict(frequency_penalty=10 ** 400), dict(presence_penalty=-10 ** 400),
+               dict(repetition_penalty=10 ** 400), dict(token_mask=fails),
+               dict(token_mask=lambda out: [2 ** 70])):
+        with pytest.raises(ValueError):
+            e.add_request("x", [1, 2], greedy(**kw))
+        with pytest.raises(ValueError):
+            e.add_request_group("g", [1, 2], greedy(**kw), 2)
+    assert not e.has_work()
+    out, = run(e, [(PROMPTS[0], greedy(3, logit_bias={3: -10 ** 400},
+                                       allowed_token_ids=(3, 5)))])
+    assert out.output_ids == [5] * 3              # a ban, as any below 32 bits
+    with pytest.raises(ValueError):
+        token_words([2 ** 70], 512)
+    rules = LogitRules(1, 8, 4, "cpu", biases=1)
+    for kw in (dict(frequency=10 ** 400), dict(allowed=[2 ** 70]),
+               dict(bias={2 ** 70: 1.0})):
+        with pytest.raises(ValueError):
+            rules.set(0, **kw)
+    rules.set(0, bias={1: -10 ** 400})
+    assert rules.bias_values[0, 0] == -math.inf
+    with pytest.raises(ValueError):
+        e.load_adapter("x", export_adapter(models[0][0])[0], 10 ** 400)
+
+
 def test_rules_on_hybrid_decoders():
     e = Engine(get_model_config("kuforax-debug"), device="cpu", dtype=torch.float32,
                kv_token_capacity=512, max_running_requests=4)
