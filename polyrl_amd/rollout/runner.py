@@ -99,7 +99,7 @@ class EngineRunner:
         try:
             with self._admin_lock():
                 self.engine.add_request(rid, input_ids, sp)
-        except ValueError:               # refused: nobody will answer
+        except BaseException:            # refused: nobody will answer
             self._futures.pop(rid, None)
             raise
         self.start()
@@ -123,7 +123,7 @@ class EngineRunner:
         try:
             with self._admin_lock():
                 self.engine.add_request_group(prefix, input_ids, sp, n)
-        except ValueError:
+        except BaseException:
             for s_ in range(n):
                 self._futures.pop(f"{prefix}-s{s_}", None)
             raise

@@ -467,6 +467,27 @@ def test_http(models, tmp_path):
     runner.stop()
 
 
+def test_refused_requests_leave_no_future(models, monkeypatch):
+    """Whatever the engine raises when it is asked, nobody is left waiting."""
+    from polyrl_amd.rollout.runner import EngineRunner
+    e = engine(models[0][1])
+    runner = EngineRunner(e)
+
+    async def go():
+        for error in (OverflowError, KeyError, TypeError, AssertionError):
+            def refuse(*a):
+                raise error
+            for name in ("add_request", "add_request_group"):
+                monkeypatch.setattr(e, name, refuse)
+            with pytest.raises(error):
+                runner.submit([1], greedy())
+            with pytest.raises(error):
+                runner.submit_group([1], greedy(), 3)
+            assert not runner._futures
+    asyncio.run(go())
+    runner.stop()
+
+
 # ---------------------------------------------------- from training to serving
 
 
