@@ -51,6 +51,12 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
                 int(t) for t in d.get("allowed_token_ids") or ()),
             adapter=str(d.get("adapter") or ""))
 
+    async def _json_object(request: Request) -> dict:
+        body = await request.json()
+        if not isinstance(body, dict):
+            raise ValueError("the body is no JSON object")
+        return body
+
     def _meta(o, include_logprobs: bool) -> dict:
         m = {"finish_reason": {"type": o.finish_reason},
              "completion_tokens": len(o.output_ids)}
@@ -67,7 +73,7 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
         try:
             sp = _sp(body.get("sampling_params", {}))
             n = int(body.get("sampling_params", {}).get("n", 1))
-        except (ValueError, TypeError, AttributeError) as e:
+        except (ValueError, TypeError, AttributeError, OverflowError) as e:
             return JSONResponse({"success": False,
                                  "message": f"sampling_params: {e}"}, 400)
         want_lp = bool(body.get("return_logprob", False))
@@ -144,22 +150,22 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
                                 403)
         from safetensors import SafetensorError
         from safetensors.torch import load, load_file
-        if request.headers.get("content-type", "").startswith(
-                "application/json"):
-            body = await request.json()
-            name, scaling = body.get("name"), body.get("scaling", 1.0)
-            read = lambda: load_file(body["path"])
-        else:
-            raw = await request.body()
-            name = request.headers.get("x-adapter-name")
-            scaling = request.headers.get("x-adapter-scaling", "1.0")
-            read = lambda: load(raw)
         try:
+            if request.headers.get("content-type", "").startswith(
+                    "application/json"):
+                body = await _json_object(request)
+                name, scaling = body.get("name"), body.get("scaling", 1.0)
+                read = lambda: load_file(body["path"])
+            else:
+                raw = await request.body()
+                name = request.headers.get("x-adapter-name")
+                scaling = request.headers.get("x-adapter-scaling", "1.0")
+                read = lambda: load(raw)
             name, scaling = str(name or ""), float(scaling)
             await asyncio.get_running_loop().run_in_executor(
                 None, lambda: runner.load_adapter(name, read(), scaling))
         except (ValueError, TypeError, KeyError, RuntimeError, OSError,
-                SafetensorError) as e:
+                OverflowError, SafetensorError) as e:
             return JSONResponse({"success": False, "message": str(e)}, 400)
         return {"success": True, "adapters": engine.adapters}
 
@@ -169,8 +175,8 @@ def create_app(engine: Engine, runner: Optional[EngineRunner] = None,
             return JSONResponse({"success": False,
                                  "message": "sender not in allowed CIDRs"},
                                 403)
-        body = await request.json()
         try:
+            body = await _json_object(request)
             await asyncio.get_running_loop().run_in_executor(
                 None, lambda: runner.unload_adapter(str(body.get("name"))))
         except (ValueError, RuntimeError) as e:

@@ -488,6 +488,37 @@ def test_refused_requests_leave_no_future(models, monkeypatch):
     runner.stop()
 
 
+def test_http_numbers_and_bodies_of_any_kind(models):
+    httpx = pytest.importorskip("httpx")
+    from polyrl_amd.rollout.runner import EngineRunner
+    from polyrl_amd.server.engine_server import create_app
+    e = engine(models[0][1])
+    runner = EngineRunner(e)
+    app = create_app(e, runner)
+    big = "1" + "0" * 400
+
+    async def go():
+        async with httpx.AsyncClient(transport=httpx.ASGITransport(
+                app=app, raise_app_exceptions=False), base_url="http://t") as c:
+            kind = {"content-type": "application/json"}
+            for sp in ('"allowed_token_ids": [%s]' % big, '"logit_bias": {"3": %s}' % big,
+                       '"logit_bias": {"%s": 1}' % big, '"allowed_token_ids": [Infinity]',
+                       '"frequency_penalty": %s' % big, '"top_k": Infinity',
+                       '"allowed_token_ids": [%d]' % 2 ** 70):
+                r = await c.post("/generate", headers=kind, content=
+                                 '{"input_ids": [1, 2], "sampling_params": {%s}}' % sp)
+                assert r.status_code == 400, sp
+            for body in ("[]", "5", "null", '"a"', "{", "",
+                         '{"name": "a", "path": "/no", "scaling": %s}' % big):
+                for where in ("/load_adapter", "/unload_adapter"):
+                    r = await c.post(where, headers=kind, content=body)
+                    assert r.status_code == 400, (where, body)
+                    assert r.json()["success"] is False
+        assert not runner._futures and not e.has_work() and not e.adapters
+    asyncio.run(go())
+    runner.stop()
+
+
 # ---------------------------------------------------- from training to serving
 
 
