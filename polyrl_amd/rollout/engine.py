@@ -539,6 +539,7 @@ class Engine:
         self._forced: Dict[str, Request] = {}
         self.rules = RequestRules(cfg.vocab_size, self.max_model_len + 1,
                                   max_running_requests, device)
+        self._graph_table = None      # the rules' tables that captured steps go by
         if self.hybrid:
             self._init_hybrid(page_size, kv_bytes_budget, kv_token_capacity,
                               seed, decode_chunk_size)
@@ -981,7 +982,7 @@ class Engine:
             (r.sampling.top_k <= 0 or r.sampling.top_k >= logits.shape[-1])
             and r.sampling.top_p >= 1.0 for r in reqs)
         tokens, lps = self._draw(logits, temp, tk, tp, seed,
-                                 self.rules.rows(reqs),
+                                 self._rule_rows(reqs),
                                  generator=self._gen, no_filter=no_filter)
         tokens_l = tokens.tolist()
         lps_l = lps.tolist()
@@ -999,6 +1000,19 @@ class Engine:
                 r.finished = True
                 r.finish_reason = "length"
             self._next_mask(r)
+
+    def _rule_rows(self, reqs: List[Request]) -> Optional[torch.Tensor]:
+        """``RequestRules.rows``.  Steps that were captured over tables which were made
+        larger go, and the old tables with them."""
+        rows = self.rules.rows(reqs)
+        table = self.rules.table
+        if self._graph_table is not table:
+            self._graph_table = table
+            self._graphs = {k: st for k, st in self._graphs.items()
+                            if st.get("rules") in (None, table)}
+            if not self._graphs:         # nothing holds their memory pool any more
+                self._graph_pool = None
+        return rows
 
     def _draw(self, logits, temp, tk, tp, seed, rows, **kw):
         """``ops.sample`` under the rules of the requests whose slots ``rows`` names (None:
@@ -1421,7 +1435,7 @@ class Engine:
         no_filter = all(
             (r.sampling.top_k <= 0 or r.sampling.top_k >= self.cfg.vocab_size)
             and r.sampling.top_p >= 1.0 for r in reqs)
-        rule_rows = self.rules.rows(reqs)
+        rule_rows = self._rule_rows(reqs)
         own = self._adapter_slots(reqs)
         index = None if own is None else torch.tensor(
             own, dtype=torch.int32, device=dev)
@@ -1500,14 +1514,10 @@ class Engine:
         # [B:Bb) are dummies writing KV into a reserved scratch slot
         Bb = decode_bucket(B) if self._decode_buckets else B
         scratch = self._decode_scratch_slot() if Bb > B else 0
-        # steps with rules or adapters are captured apart from those without, and anew
-        # when the rules' tables were made larger
+        # steps with rules or adapters are captured apart from those without
         key = Bb if rule_rows is None and index is None else \
             (Bb, rule_rows is not None, index is not None)
         st = self._graphs.get(key)
-        if st is not None and rule_rows is not None \
-                and st["rules"] is not self.rules.table:
-            st = None
         if st is None:
             st = {
                 "tokens": torch.zeros(Bb, dtype=torch.int64, device=dev),

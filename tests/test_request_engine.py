@@ -337,6 +337,27 @@ def test_more_requests_than_slots(models):
     assert not e.rules._slots
 
 
+def test_captured_steps_go_with_their_table(models):
+    """When the rules' tables are made larger the old ones are let go, with every step that
+    was captured over them; the other steps stay."""
+    e = engine(models[0][1])
+    run(e, [(PROMPTS[0], greedy(3, logit_bias={5: 1.0}))])
+    old = weakref.ref(e.rules.table)
+    with no_collector():
+        e._graphs = {4: {"rules": None}, (4, True, False): {"rules": old()},
+                     (2, True, True): {"rules": old()}, (2, False, True): {"rules": None}}
+        e._graph_pool = (0, 1)
+        run(e, [(PROMPTS[0], greedy(3, logit_bias={6: 1.0}))])
+        assert old() is e.rules.table and len(e._graphs) == 4
+        run(e, [(PROMPTS[0], greedy(3, logit_bias={t: 1.0 for t in range(9)}))])
+        assert list(e._graphs) == [4, (2, False, True)] and e._graph_pool == (0, 1)
+        assert old() is None
+        # a pool that no captured step holds any more cannot be taken again
+        e._graphs = {(4, True, False): {"rules": e.rules.table}}
+        run(e, [(PROMPTS[0], greedy(3, logit_bias={t: 1.0 for t in range(99)}))])
+        assert e._graphs == {} and e._graph_pool is None
+
+
 def test_rules_that_cannot_hold(models):
     e = engine(models[0][1])
     inf = math.inf
@@ -722,6 +743,25 @@ def test_captured_steps_go_with_their_engine(tiny):
         gone = [weakref.ref(e)] + [weakref.ref(t["tokens"]) for t in e._graphs.values()]
         del e
         assert not any(r() is not None for r in gone)
+
+
+@pytest.mark.gpu
+def test_steps_are_captured_anew_for_a_larger_table(tiny):
+    jobs = [(p, greedy(20, logit_bias={3: 2.0})) for p, _ in mixed_jobs(3)]
+    more = [(p, greedy(20, logit_bias={t: 2.0 for t in range(40)})) for p, _ in jobs]
+    want = [run(gpu_engine(tiny, True), j) for j in (jobs, more)]
+    for plain in (False, True):                   # with a step that stays, and without
+        e = gpu_engine(tiny, True)
+        if plain:
+            run(e, [(p, greedy(20)) for p, _ in jobs])
+        for _ in range(2):
+            assert [o.output_ids for o in run(e, jobs)] == \
+                [o.output_ids for o in want[0]]
+        for _ in range(2):
+            assert [o.output_ids for o in run(e, more)] == \
+                [o.output_ids for o in want[1]]
+        assert e.enable_hip_graphs and e._graphs
+        assert all(st["rules"] in (None, e.rules.table) for st in e._graphs.values())
 
 
 @pytest.mark.gpu
