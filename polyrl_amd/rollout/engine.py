@@ -17,7 +17,9 @@ from __future__ import annotations
 import contextlib
 import gc
 import math
+import threading
 import time
+import types
 import weakref
 from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional
@@ -94,19 +96,29 @@ DECODE_BUCKETS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128,
                   192, 256)
 
 
+# captures under way in this process, and whether the collector was on before them
+_captures = types.SimpleNamespace(lock=threading.Lock(), n=0, collects=False)
+
+
 @contextlib.contextmanager
 def _captured(graph, pool=None):
     """``torch.cuda.graph`` without the garbage collector: a graph that it found then
     (of an engine that was let go) would be destroyed while the stream captures, which
-    the runtime forbids, and an error in a destructor ends the process."""
-    on = gc.isenabled()
-    gc.disable()
+    the runtime forbids, and an error in a destructor ends the process.  Of captures in
+    several threads the first one turns it off and the last one on again."""
+    with _captures.lock:
+        if _captures.n == 0:
+            _captures.collects = gc.isenabled()
+            gc.disable()
+        _captures.n += 1
     try:
         with torch.cuda.graph(graph, pool=pool):
             yield
     finally:
-        if on:
-            gc.enable()
+        with _captures.lock:
+            _captures.n -= 1
+            if _captures.n == 0 and _captures.collects:
+                gc.enable()
 
 
 def decode_bucket(b: int) -> int:

@@ -734,6 +734,36 @@ def test_no_collection_while_a_step_is_captured(monkeypatch, on):
         gc.enable()
 
 
+@pytest.mark.parametrize("on", [True, False])
+def test_no_collection_while_another_thread_captures(monkeypatch, on):
+    """Two engines that capture at once: the collector is off until both are done."""
+    import threading
+
+    from polyrl_amd.rollout import engine as module
+    monkeypatch.setattr(torch.cuda, "graph",
+                        lambda g, pool=None: contextlib.nullcontext())
+    inside, leave, seen = threading.Event(), threading.Event(), []
+
+    def second():
+        with module._captured(None):
+            inside.set()
+            assert leave.wait(30)
+            seen.append(gc.isenabled())
+    thread = threading.Thread(target=second)
+    try:
+        (gc.enable if on else gc.disable)()
+        with module._captured(None):
+            thread.start()
+            assert inside.wait(30)
+        assert not gc.isenabled()                 # the other one goes on
+        leave.set()
+        thread.join(30)
+        assert seen == [False] and gc.isenabled() == on
+    finally:
+        leave.set()
+        gc.enable()
+
+
 @pytest.mark.gpu
 def test_captured_steps_go_with_their_engine(tiny):
     with no_collector():
