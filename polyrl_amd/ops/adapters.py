@@ -75,5 +75,10 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
             or not 1 <= a.shape[2] <= MOST_RANK or a.shape[3] >= 1 << 20:
         raise ValueError(f"adapter_add: 1 to {MOST_PARTS} parts, ranks 1 to "
                          f"{MOST_RANK}, inner widths below 2^20")
+    if out is not None:
+        in_place = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
+        if any(ref.rows_overlap(out, t)
+               for t in ((x, a, b) if in_place else (y, x, a, b))):
+            raise ValueError("adapter_add: out on top of an operand")
     res = ref.adapter_add(y, x, a, b, scale, plan.index, widths, ranks)
     return res if out is None else out.copy_(res)

@@ -27,6 +27,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include "common.h"
+#include "rows_overlap.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
@@ -723,10 +724,16 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                 "adapter_add: tensors of one type and device");
   for (const auto& t : {out, y, x})
     TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, "adapter_add: rows of adjacent numbers");
-  TORCH_CHECK((out.data_ptr() != y.data_ptr() || out.strides() == y.strides()) &&
-                  (T <= 1 || out.stride(0) >= N),
-              "adapter_add: out is y or apart from it, its rows from each other");
   TORCH_CHECK(a.is_contiguous() && b.is_contiguous(), "adapter_add: contiguous a and b");
+  TORCH_CHECK(T <= 1 || out.stride(0) >= N,
+              "adapter_add: out is y or apart from it, its rows from each other");
+  if (into.has_value()) {
+    const bool in_place = out.data_ptr() == y.data_ptr() && out.strides() == y.strides();
+    TORCH_CHECK(in_place || !rows_overlap(out, y),
+                "adapter_add: out is y or apart from it, its rows from each other");
+    for (const auto& t : {x, a, b})
+      TORCH_CHECK(!rows_overlap(out, t), "adapter_add: out on top of an operand");
+  }
   TORCH_CHECK(scale.device() == y.device() && scale.scalar_type() == torch::kFloat32 &&
                   scale.is_contiguous() && scale.numel() == S,
               "adapter_add: scale (S) fp32");

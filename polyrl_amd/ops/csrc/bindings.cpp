@@ -2,6 +2,8 @@
 #include <torch/extension.h>
 #include <vector>
 
+#include "rows_overlap.h"
+
 void rmsnorm(torch::Tensor out, torch::Tensor x, torch::Tensor weight,
              double eps);
 void fused_add_rmsnorm(torch::Tensor out, torch::Tensor residual,
@@ -182,6 +184,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dropout_train", &dropout_train, "seeded dropout, differentiable, no mask kept");
   m.def("adjust_logits", &adjust_logits,
         "penalties, biases and allowed tokens on a step's logits");
+  m.def("rows_overlap", &rows_overlap, "whether two operands share memory");
   m.def("append_tokens", &append_tokens, "tokens at the ends of histories");
   m.def("adapter_plan", &adapter_plan, "rows in tiles of one adapter each");
   m.def("adapter_add", &adapter_add, "y + s B (A x) by each row's adapter");

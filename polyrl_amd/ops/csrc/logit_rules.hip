@@ -23,6 +23,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <c10/core/DeviceGuard.h>
 
+#include "rows_overlap.h"
 #include "vocab_row.h"
 
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
@@ -267,8 +268,8 @@ void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
   TORCH_CHECK((V <= 1 || (logits.stride(1) == 1 && out.stride(1) == 1)) &&
                   V < (1L << 30),
               "adjust_logits: rows of adjacent numbers");
-  TORCH_CHECK((out.data_ptr() != logits.data_ptr() || out.strides() == logits.strides()) &&
-                  (N <= 1 || out.stride(0) >= V),
+  TORCH_CHECK(((out.data_ptr() == logits.data_ptr() && out.strides() == logits.strides()) ||
+               !rows_overlap(out, logits)) && (N <= 1 || out.stride(0) >= V),
               "adjust_logits: out is logits or apart from it, its rows from each other");
   for (const auto& t : {rows, history, prompt_len, total_len, bias_tokens, mask, masked})
     check_ints(t, logits, "adjust_logits");

@@ -205,6 +205,30 @@ def varlen_lse(q, k, cu_seqlens_q, cu_seqlens_k, scale, causal=True):
     return out
 
 
+def rows_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two operands share memory: rows of adjacent numbers (N, W) that may lie
+    apart, or contiguous tensors.  The rule of rows_overlap.h."""
+    def rows(t):
+        size = t.element_size()
+        if t.dim() != 2 or t.numel() == 0 or t.shape[0] == 1:
+            return t.data_ptr(), 1, 0, t.numel() * size
+        return t.data_ptr(), t.shape[0], t.stride(0) * size, t.shape[1] * size
+    p, q = rows(a), rows(b)
+    ends = [at + (n - 1) * pitch + width for at, n, pitch, width in (p, q)]
+    if not p[3] or not q[3] or ends[0] <= q[0] or ends[1] <= p[0]:
+        return False
+    if p[2] == q[2] == 0:
+        return True
+    (at0, n0, pitch0, w0), (at1, n1, pitch1, w1) = (q, p) if q[2] == 0 else (p, q)
+    same = pitch0 == pitch1
+    for i in range(1 if same else n0):
+        d = at0 + i * pitch0 - at1
+        low, high = (d - w1) // pitch1 + 1, -(-(d + w0) // pitch1) - 1
+        if max(low, 1 - n0 if same else 0) <= min(high, n1 - 1):
+            return True
+    return False
+
+
 # ------------------------------------------------------- adapters of requests
 
 

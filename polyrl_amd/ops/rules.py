@@ -167,6 +167,9 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, rows: torch.Tensor,
                           rules.frequency, rules.presence, rules.bias_tokens,
                           rules.bias_values, rules.mask, rules.masked)
         return out
+    if out is not None and ref.rows_overlap(out, logits) and (
+            out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+        raise ValueError("adjust_logits: out is logits or apart from it")
     res = ref.adjust_logits(logits, rules, rows)
     return res if out is None else out.copy_(res)
 

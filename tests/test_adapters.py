@@ -265,6 +265,62 @@ def test_captured(T):
         assert torch.equal(replayed, step())
 
 
+def test_which_views_share_memory():
+    """Both forms of the rule against the sets of addresses, over views of one buffer."""
+    from polyrl_amd.ops import ref
+    buf = torch.zeros(64)
+    at = torch.arange(64)
+    g = torch.Generator().manual_seed(0)
+    pick = lambda low, high: int(torch.randint(low, high + 1, (1,), generator=g))
+    seen = [0, 0]
+    for _ in range(4000):
+        views = []
+        for _ in range(2):
+            n, width, pitch = pick(0, 4), pick(0, 5), pick(0, 9)
+            first = pick(0, 63 - 3 * 9 - 5)
+            views.append(((n, width), (pitch, 1), first))
+        a, b = (buf.as_strided(*v) for v in views)
+        one, two = (set(at.as_strided(*v).flatten().tolist()) for v in views)
+        want = bool(one & two)
+        seen[want] += 1
+        assert ref.rows_overlap(a, b) is want, views
+        if ops.extension_loaded():
+            assert ops._EXT.rows_overlap(a, b) is want, views
+    assert min(seen) > 500
+    flat = buf[:24].view(2, 3, 4)                 # contiguous tensors of any rank
+    for off, want in ((20, True), (24, False)):
+        assert ref.rows_overlap(buf[off:off + 8].view(2, 4), flat) is want
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_outputs_on_top_of_operands(dev):
+    """Shifted by rows or columns, or over x or the adapters: refused.  Rows between y's,
+    columns beside them and y itself are places like others."""
+    T, N, K, r, S = 6, 16, 32, 8, 2
+    g = torch.Generator().manual_seed(0)
+    pool = torch.randn(4096, generator=g).to(dev)
+    y = pool[64:].as_strided((T, N), (40, 1))
+    x = pool[1024:1024 + T * K].view(T, K)
+    a = pool[2048:2048 + S * r * K].view(S, 1, r, K)
+    b = pool[3072:3072 + S * N * r].view(S, N, r)
+    scale = torch.ones(S, device=dev)
+    index = torch.arange(T, dtype=torch.int32) % (S + 1) - 1
+    plan = ops.adapter_plan(index.to(dev), S)
+    keep = pool.clone()
+    at = lambda first, pitch=40: pool.as_strided((T, N), (pitch, 1), first)
+    for out in (at(64 + 40), at(64 - 40), at(64 + 15), at(64 - 1), at(64, 41), at(66, 16),
+                at(1024, N), at(1024 + T * K - 1), at(2048, N), at(3072 + 5, 33)):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.adapter_add(y, x, a, b, scale, plan, out=out)
+    assert torch.equal(pool, keep)                # refused before anything is written
+    want = ops.adapter_add(y, x, a, b, scale, plan)
+    for first in (64 + 16, 64 - 16, 64 + 24, 64 + T * 40, 1024 + T * K, 64):
+        pool.copy_(keep)
+        out = at(first)
+        assert ops.adapter_add(y, x, a, b, scale, plan, out=out) is out
+        assert torch.equal(out, want), first
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_refusals(dev):
     y, x, a, b, scale = make(dev, BF16, 6, 32, (16,), 8, 2)

@@ -249,6 +249,32 @@ def test_captured():
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_outputs_on_top_of_logits(dev, dtype):
+    """A view of the logits' memory that is not the logits is refused where it shares
+    a number with them, and a place like others where it does not."""
+    N, V = 5, 40
+    pool = torch.randn(2048, generator=torch.Generator().manual_seed(0)).to(dtype).to(dev)
+    at = lambda first, pitch=96: pool.as_strided((N, V), (pitch, 1), first)
+    logits, rules = at(256), ops.LogitRules(2, V, 6, dev)
+    rules.set(0, prompt=[3], output=[4, 4], repetition=1.5, frequency=0.5)
+    rules.set(1, allowed=range(7))
+    rows = torch.tensor([0, 1, -1, 0, 1], dtype=torch.int32, device=dev)
+    keep = pool.clone()
+    for out in (at(256 + 96), at(256 - 96), at(256 + 8), at(256 - 39), at(256, 48),
+                at(256, 104), at(300, 47)):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.adjust_logits(logits, rules, rows, out=out)
+    assert torch.equal(pool, keep)
+    want = ops.adjust_logits(logits, rules, rows)
+    for first in (256 + 40, 256 - 40, 256 + 51, 256 + 5 * 96, 256):
+        pool.copy_(keep)
+        out = at(first)
+        assert ops.adjust_logits(logits, rules, rows, out=out) is out
+        assert torch.equal(out, want), first
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_refusals(dev):
     rules = ops.LogitRules(2, 40, 6, dev, biases=1)
     for kw in (dict(repetition=0.0), dict(repetition=-1.0),
