@@ -86,7 +86,6 @@ __global__ __launch_bounds__(NT) void logit_rules_kernel(
   T* to = out + row * ld_out;
   // groups of VEC tokens; the first one of a row that starts inside a word is short
   const int lead = WIDE ? in.lead : 0, ahead = WIDE ? 1 : 0;
-  const int all = ahead + (V - lead + VEC - 1) / VEC;
   const int g0 = part * NT * U;
   const int base = lead + (g0 - ahead) * VEC;     // the chunk's first token, may be < 0
   // LDS word of the chunk's token t: a thread's VEC tokens in two halves (of 8), so that
@@ -236,11 +235,11 @@ __global__ __launch_bounds__(256) void append_tokens_kernel(
       int before = 0, behind = 0;
       for (int j = 0; j < N; ++j)
         if (rows[j] == s) j < i ? ++before : j > i ? ++behind : 0;
-      const long at = (long)min(max(total_len[s], 0), cap) + before;
+      const long had = max(total_len[s], 0), at = had + before;
       if (step == 0) {
         const int64_t t = tokens[i];
         if (at < cap) history[(long)s * cap + at] = t >= 0 && t < (1L << 31) ? (int)t : -1;
-      } else if (behind == 0) {
+      } else if (behind == 0 && had < cap) {
         total_len[s] = (int)min(at + 1, (long)cap);
       }
     }

@@ -18,6 +18,7 @@ from . import ref
 
 MOST_TOKENS = (1 << 19) - 1      # of a history
 MOST_BIASES = (1 << 12) - 1      # of a slot
+MOST_ROWS = 1 << 14              # whose tokens are recorded at a time (one block does)
 
 
 def token_words(tokens, vocab: int) -> np.ndarray:
@@ -177,7 +178,9 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, rows: torch.Tensor,
 def append_tokens(rules: LogitRules, rows: torch.Tensor,
                   tokens: torch.Tensor) -> None:
     """tokens (N,) int64 to the histories of slots ``rows`` (N,) int32, those of one slot in
-    their order.  A full history stays as it is."""
+    their order.  A full history stays as it is.  At most 16384 rows."""
+    if rows.numel() > MOST_ROWS:
+        raise ValueError(f"append_tokens: at most {MOST_ROWS} rows")
     if rows.dtype != torch.int32 or rows.dim() != 1 \
             or tokens.dtype != torch.int64 or tokens.shape != rows.shape:
         raise ValueError("append_tokens: rows (N,) int32, tokens (N,) int64")

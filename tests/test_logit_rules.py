@@ -205,6 +205,22 @@ def test_append(dev):
     assert rules.history[2, :350].tolist() == list(range(1, 700, 2))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_append_to_lengths_outside_of_the_history(dev):
+    """A full history stays as it is, its length too, whatever a program wrote there; a
+    negative length is an empty history."""
+    rules = ops.LogitRules(5, 40, 3, dev)
+    rules.total_len.copy_(torch.tensor([3, 9, -4, 2, 7], dtype=torch.int32))
+    rows = torch.tensor([0, 1, 2, 3, 3, 1, 3], dtype=torch.int32, device=dev)
+    ops.append_tokens(rules, rows, torch.arange(10, 17, device=dev))
+    assert rules.total_len.tolist() == [3, 9, 1, 3, 7]
+    assert rules.history.tolist() == [[-1] * 3, [-1] * 3, [12, -1, -1], [-1, -1, 13],
+                                      [-1] * 3]
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.append_tokens(rules, torch.zeros(16385, dtype=torch.int32, device=dev),
+                          torch.zeros(16385, dtype=torch.int64, device=dev))
+
+
 @pytest.mark.gpu
 def test_captured():
     """A decode step with rules: logits, token, history; replayed as it runs."""
