@@ -65,14 +65,18 @@ def fused_add_rmsnorm(x: torch.Tensor, residual: torch.Tensor,
     return ref.fused_add_rmsnorm(x, residual, weight, eps)
 
 
-def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
-    """gate/up may be strided row views into a fused gate_up projection."""
+def silu_mul(gate: torch.Tensor, up: torch.Tensor,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gate/up may be strided row views into a fused gate_up projection; ``out``:
+    contiguous, apart from both."""
     if gate.is_cuda:
         ext = _require_ext()
-        out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+        if out is None:
+            out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
         ext.silu_mul(out, gate, up)
         return out
-    return ref.silu_mul(gate, up)
+    res = ref.silu_mul(gate, up)
+    return res if out is None else out.copy_(res)
 
 
 def linear_takes(x: torch.Tensor, w: torch.Tensor) -> bool:
@@ -104,13 +108,15 @@ def linear_rows(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return _require_ext().linear_rows(x, w) if x.is_cuda else x @ w.t()
 
 
-def linear_swiglu(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+def linear_swiglu(x: torch.Tensor, w: torch.Tensor,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """silu(x @ Wg.T) * (x @ Wu.T) with w = [Wg; Wu], (2 I, H): the gated MLP's
-    first half without its intermediate rows (no autograd)."""
+    first half without its intermediate rows (no autograd).  ``out``: contiguous, apart
+    from both."""
     if x.is_cuda:
-        return _require_ext().linear_swiglu(x, w)
+        return _require_ext().linear_swiglu(x, w, out)
     gate, up = (x @ w.t()).chunk(2, dim=-1)
-    return ref.silu_mul(gate, up)
+    return silu_mul(gate, up, out)
 
 
 # ---------------------------------------------------------------------- RoPE

@@ -10,7 +10,8 @@ void fused_add_rmsnorm(torch::Tensor out, torch::Tensor residual,
                        torch::Tensor x, torch::Tensor weight, double eps);
 void silu_mul(torch::Tensor out, torch::Tensor gate, torch::Tensor up);
 torch::Tensor linear_rows(torch::Tensor x, torch::Tensor w);
-torch::Tensor linear_swiglu(torch::Tensor x, torch::Tensor w);
+torch::Tensor linear_swiglu(torch::Tensor x, torch::Tensor w,
+                            const c10::optional<torch::Tensor>& out);
 bool linear_rows_pays(long M, long N, long K);
 std::vector<long> product_rows(long M, long cols, long K, long least);
 void linear_rows_add(torch::Tensor out, torch::Tensor x, torch::Tensor w);
@@ -140,7 +141,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_rows_add", &linear_rows_add, "out += x W^T, rounded once");
   m.def("linear_rows_pays", &linear_rows_pays, "linear_rows for the library's product");
   m.def("product_rows", &product_rows, "row parts of a product's tiles, their cost");
-  m.def("linear_swiglu", &linear_swiglu, "SiLU(x Wg^T) * (x Wu^T)");
+  m.def("linear_swiglu", &linear_swiglu, "SiLU(x Wg^T) * (x Wu^T)", py::arg("x"),
+        py::arg("w"), py::arg("out") = py::none());
   m.def("rope_inplace", &rope_inplace, "NEOX RoPE in place (table-driven)");
   m.def("rope_kv_append", &rope_kv_append,
         "NEOX RoPE in place on q, k + paged KV cache rows, one launch");

@@ -198,6 +198,11 @@ void silu_mul(torch::Tensor out, torch::Tensor gate, torch::Tensor up) {
   TORCH_CHECK(gate.is_cuda() && gate.dtype() == torch::kBFloat16);
   TORCH_CHECK(out.is_contiguous());
   TORCH_CHECK(gate.dim() == 2 && up.dim() == 2);
+  TORCH_CHECK(out.sizes() == gate.sizes() && up.sizes() == gate.sizes() &&
+                  out.dtype() == gate.dtype() && up.dtype() == gate.dtype() &&
+                  out.device() == gate.device() && up.device() == gate.device() &&
+                  ((uintptr_t)out.data_ptr() & 15) == 0,
+              "silu_mul: gate, up and out of one shape, bf16, on one device");
   TORCH_CHECK(gate.stride(1) == 1 && up.stride(1) == 1,
               "inner dim must be contiguous");
   const long rows = gate.size(0);

@@ -30,6 +30,7 @@
 #include <ATen/hip/HIPContext.h>
 
 #include "product_tile.h"
+#include "rows_overlap.h"
 
 namespace {
 
@@ -233,7 +234,8 @@ Part part(const torch::Tensor* out, const torch::Tensor& w, long first, long n) 
 }
 
 template <bool GLU>
-torch::Tensor linear_prompt(const torch::Tensor& x, const torch::Tensor& w) {
+torch::Tensor linear_prompt(const torch::Tensor& x, const torch::Tensor& w,
+                            const c10::optional<torch::Tensor>& into = c10::nullopt) {
   for (const auto* t : {&x, &w})
     TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->dim() == 2 &&
                     t->is_contiguous() && t->dtype() == torch::kBFloat16 &&
@@ -244,7 +246,14 @@ torch::Tensor linear_prompt(const torch::Tensor& x, const torch::Tensor& w) {
                   K < (1L << 20) && N < (1L << 25) && M < (1L << 30),
               "linear: inner numbers in 64s, the weight's rows in 256s, outputs "
               "below 2^25");
-  auto out = torch::empty({M, N}, x.options());
+  torch::Tensor out = into.has_value() ? *into : torch::empty({M, N}, x.options());
+  TORCH_CHECK(out.dim() == 2 && out.size(0) == M && out.size(1) == N &&
+                  out.device() == x.device() && out.dtype() == torch::kBFloat16 &&
+                  out.is_contiguous() && ((uintptr_t)out.data_ptr() & 15) == 0,
+              "linear: a contiguous bf16 output of the result's shape");
+  if (into.has_value())
+    TORCH_CHECK(!rows_overlap(out, x) && !rows_overlap(out, w),
+                "linear: an output on top of an operand");
   if (GLU)
     launch_linear<GATED>((bf16_t*)out.data_ptr(), x,
                          {{part(nullptr, w, 0, N), part(nullptr, w, N, N)}}, N / 128);
@@ -336,8 +345,9 @@ void linear_rows_add(torch::Tensor out, torch::Tensor x, torch::Tensor w) {
 }
 
 // x (M, K), w (2 N, K): rows of the gate, then of the up projection
-torch::Tensor linear_swiglu(torch::Tensor x, torch::Tensor w) {
-  return linear_prompt<true>(x, w);
+torch::Tensor linear_swiglu(torch::Tensor x, torch::Tensor w,
+                            const c10::optional<torch::Tensor>& out) {
+  return linear_prompt<true>(x, w, out);
 }
 
 namespace {

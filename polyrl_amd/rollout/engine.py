@@ -80,13 +80,18 @@ def _gate_up(x: torch.Tensor, w: torch.Tensor, search: bool = True
     70.9, 276, 452; 2048 -> 8192 34.1, 51.8, 256, 391 and 44.7, 69.0, 316, 472; 4096
     -> 14336 117, 183, 868, 1301 and 131, 207, 996, 1408).  Few outputs of wide
     models leave most of the chip idle."""
-    if x.shape[0] > 512 and (
-            x.shape[1] <= 1536 or x.shape[1] <= 2048 and x.shape[0] < 8192
-            or x.shape[0] * w.shape[0] >= 1 << 23) and ops.linear_takes(x, w):
+    if _is_one_kernel(x, w):
         return ops.linear_swiglu(x, w)
     i = w.shape[0] // 2
     gate_up = _mm_nt(x, w, search)
     return ops.silu_mul(gate_up.narrow(1, 0, i), gate_up.narrow(1, i, i))
+
+
+def _is_one_kernel(x: torch.Tensor, w: torch.Tensor) -> bool:
+    """Whether ``_gate_up`` has both products and the activation in one kernel."""
+    return x.shape[0] > 512 and (
+        x.shape[1] <= 1536 or x.shape[1] <= 2048 and x.shape[0] < 8192
+        or x.shape[0] * w.shape[0] >= 1 << 23) and ops.linear_takes(x, w)
 
 
 # graphed-decode batch buckets (POLYRL_DECODE_BUCKETS=1): capture counts
@@ -375,16 +380,44 @@ class InferenceModel:
         return True
 
     # ------------------------------------------------------------- forward
+    def gate_up_adapted(self, li: int, x: torch.Tensor, index: torch.Tensor, plan,
+                        plain: Optional[int], behind=None, search: bool = True
+                        ) -> torch.Tensor:
+        """``_gate_up`` of a layer with every row's adapter.  Adapters come before the
+        activation, so that their rows' gate and up are rounded to the model's type in
+        between, once by the product and once by the sum; rows without one have what
+        ``_gate_up`` has for a step of this size, where it is one kernel 32 bits.
+        ``plain``: rows without one, if they are the first; ``behind``: the plan of those
+        behind them."""
+        w = self.layers[li].w_gate_up
+        i = w.shape[0] // 2
+
+        def adapted(x, plan, search, out=None):
+            gate_up = _mm_nt(x, w, search)
+            self.adapters.add(li, "gate_up", gate_up, x, plan)
+            return ops.silu_mul(gate_up.narrow(1, 0, i), gate_up.narrow(1, i, i),
+                                out)
+        if plain == 0 or not _is_one_kernel(x, w):
+            return adapted(x, plan, search)
+        if plain is None:                # rows in any order: each has both
+            return torch.where((index < 0).unsqueeze(1), ops.linear_swiglu(x, w),
+                               adapted(x, plan, search))
+        act = x.new_empty(x.shape[0], i)
+        ops.linear_swiglu(x[:plain], w, out=act[:plain])
+        adapted(x[plain:], behind, False, act[plain:])
+        return act
+
     @torch.no_grad()
     def forward_tokens(self, token_ids: torch.Tensor, positions: torch.Tensor,
                        kv: PagedKVCache, slot_mapping: torch.Tensor,
                        attn_fn, rows: Optional[torch.Tensor] = None,
-                       adapter_index: Optional[torch.Tensor] = None
-                       ) -> torch.Tensor:
+                       adapter_index: Optional[torch.Tensor] = None,
+                       plain: Optional[int] = None) -> torch.Tensor:
         """Shared trunk: embed -> L x (norm, qkv, rope, kv-append, attn(fn),
         o-proj, norm, mlp) -> final norm.  Returns hidden (N, H), or of the
         tokens that ``rows`` names.  ``adapter_index`` (N,) int32: the adapter
-        of every token, -1 for none."""
+        of every token, -1 for none; ``plain``: how many tokens have none, if they
+        are the first ones."""
         if self.cfg.arch == "gpt2":
             hidden = self._forward_tokens_gpt2(token_ids, positions, kv,
                                                slot_mapping, attn_fn)
@@ -405,11 +438,14 @@ class InferenceModel:
         # prompts' projections add to the residual themselves, from 2^22 outputs on:
         # fewer wait for the old numbers longer than the norm behind them gains
         # (outputs of 1024: 3072 and 4096 rows +4 and +1%, 8192 -5; of 4096, 1300 and
-        # 2048 rows +2 and -2, 6145 -4)
+        # 2048 rows +2 and -2, 6145 -4).  Beside adapters too, so that rows without one
+        # have the same bits: rows with one then round the residual twice, by the product
+        # and by the adapters' sum, 2^-9 of it each
         adds = tp == 1 and residual.numel() >= 1 << 22
         # every projection's adapters, by one grouping of the step's rows
         plan = None if adapter_index is None else \
             self.adapters.plan(adapter_index)
+        behind = self.adapters.plan(adapter_index[plain:]) if plain else None
 
         def adapt(li, proj, y, x):
             if plan is not None:
@@ -439,8 +475,9 @@ class InferenceModel:
                 attn_out = attn_out.index_select(0, rows)
                 residual = residual.index_select(0, rows)
                 if plan is not None:
-                    plan = self.adapters.plan(
-                        adapter_index.index_select(0, rows))
+                    adapter_index = adapter_index.index_select(0, rows)
+                    plan = self.adapters.plan(adapter_index)
+                    plain = None                      # (rows in any order)
             if adds and not few and _takes_rows(attn_out, lw.wo):
                 ops.linear_rows_add(residual, attn_out, lw.wo)
                 adapt(li, "o", residual, attn_out)
@@ -453,12 +490,9 @@ class InferenceModel:
                     hidden, residual, lw.post_ln, cfg.rms_norm_eps)
             if plan is None:
                 act = _gate_up(hidden, lw.w_gate_up, not few)
-            else:                       # the adapters come before the activation
-                gate_up = _mm_nt(hidden, lw.w_gate_up, not few)
-                adapt(li, "gate_up", gate_up, hidden)
-                i = gate_up.shape[1] // 2
-                act = ops.silu_mul(gate_up.narrow(1, 0, i),
-                                   gate_up.narrow(1, i, i))
+            else:
+                act = self.gate_up_adapted(li, hidden, adapter_index, plan, plain,
+                                           behind, not few)
             if adds and not few and _takes_rows(act, lw.w_down):
                 ops.linear_rows_add(residual, act, lw.w_down)
                 adapt(li, "down", residual, act)
@@ -1268,6 +1302,19 @@ class Engine:
         """Each request's tokens [start, start+len) against its cached history
         (dense decoders); hidden rows of those of them, counted through the
         requests, that ``rows`` names."""
+        own, plain = self._adapter_slots(reqs), None
+        if own is not None and sum(lens) > 512:
+            # requests without adapter first: their gate and up stay one kernel's
+            first = np.cumsum([0] + list(lens))
+            order = sorted(range(len(reqs)), key=lambda i: own[i] >= 0)
+            reqs, starts, lens, own = ([t[i] for i in order]
+                                       for t in (reqs, starts, lens, own))
+            if rows:
+                at = np.searchsorted(first, rows, side="right") - 1
+                now = np.empty(len(order), np.int64)
+                now[order] = np.cumsum([0] + lens[:-1])
+                rows = now[at] + np.asarray(rows) - first[at]
+            plain = sum(n for n, s in zip(lens, own) if s < 0)
         cu_q, cu_k = [0], [0]
         for start, take in zip(starts, lens):
             cu_q.append(cu_q[-1] + take)
@@ -1294,7 +1341,6 @@ class Engine:
             parts.append(np.concatenate(
                 [self.kv.slots_for_host(sid, 0, s + m)
                  for sid, s, m in zip(sids, starts, lens)]))
-        own = self._adapter_slots(reqs)
         if own is not None:
             parts.append(np.repeat(np.asarray(own, np.int32), lens))
         tokens, positions, slots, cu_q_t, cu_k_t, rows_t, *hist = \
@@ -1310,7 +1356,7 @@ class Engine:
                                                 self._scale, causal=True)
 
         return self.model.forward_tokens(tokens.long(), positions, self.kv,
-                                         slots, attn_fn, rows_t, index)
+                                         slots, attn_fn, rows_t, index, plain)
 
     def _upload(self, parts) -> List[torch.Tensor]:
         """int32 arrays as device tensors, through one pinned buffer and one

@@ -2,12 +2,14 @@
 HTTP facade and from a trained adapter to a served one."""
 import asyncio
 import contextlib
+import dataclasses
 import gc
 import math
 import os
 import subprocess
 import sys
 import weakref
+from unittest import mock
 
 import numpy as np
 import pytest
@@ -94,6 +96,26 @@ def test_adapters_of_one_batch_are_the_merged_models(models):
         assert o.output_ids == w.output_ids
         assert np.allclose(o.output_logprobs, w.output_logprobs, atol=2e-4)
     assert want[0][0].output_ids != want[1][0].output_ids
+
+
+def test_long_prompt_steps_of_any_order(models):
+    """Steps of many rows put requests without adapter first: every request gets its own
+    result, cached histories and forced tokens included."""
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 512, (n,), generator=g).tolist()
+               for n in (300, 7, 150, 90, 1, 260, 40)]
+    names = ("one", "", "two", "", "two", "", "one")
+    want = {}
+    for name, sd in (("", models[0][1]), ("one", merged_state_dict(models[0][0])),
+                     ("two", merged_state_dict(models[1][0]))):
+        want[name] = run(engine(sd, max_num_batched_tokens=2048),
+                         [(p, greedy(4)) for p in prompts])
+    for tokens in (2048, 600):                    # at once, and in portions
+        e = serving(models, max_num_batched_tokens=tokens, max_running_requests=16)
+        outs = run(e, [(p, greedy(4, adapter=a)) for p, a in zip(prompts, names)])
+        for i, (o, a) in enumerate(zip(outs, names)):
+            assert o.output_ids == want[a][i].output_ids
+            assert np.allclose(o.output_logprobs, want[a][i].output_logprobs, atol=2e-4)
 
 
 def test_groups_and_prefix_cache_keep_adapters_apart(models):
@@ -808,6 +830,73 @@ def test_plain_requests_keep_their_results_beside_others(tiny):
         if i % 3:
             assert a.output_ids == b.output_ids
             assert a.output_logprobs == b.output_logprobs
+
+
+@pytest.fixture(scope="module")
+def whole():
+    """(an engine's maker, models) of llama-tiny with feed-forward rows in whole tiles, which
+    prompts take in one kernel with the activation"""
+    cfg = dataclasses.replace(get_model_config("llama-tiny"), intermediate_size=768)
+
+    def here(f):
+        def call(*args, **kw):
+            with mock.patch.object(sys.modules[__name__], "get_model_config",
+                                   lambda name: cfg):
+                return f(*args, **kw)
+        return call
+    models = [here(trained)(1, r=16),
+              here(trained)(2, r=5, targets=("q_proj", "v_proj", "gate_proj",
+                                             "down_proj"))]
+    return lambda: here(gpu_engine)(models, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [(300, 700, 90), (513, 20), (900, 4, 1200, 300)])
+def test_plain_prompts_keep_their_results_beside_adapters(whole, lens):
+    """A prompt without adapter in a step of many rows has the bits that it has beside
+    prompts that name none: its gate and up stay in 32 bits until the activation."""
+    g = torch.Generator().manual_seed(1)
+    prompts = [torch.randint(0, 1024, (n,), generator=g).tolist() for n in lens]
+    want = run(whole(), [(p, greedy(1)) for p in prompts])
+    for names in (("", "one", "two", ""), ("two", "", "one", "two"),
+                  ("", "", "one", "")):
+        got = run(whole(), [(p, greedy(1, adapter=a))
+                            for p, a in zip(prompts, names)])
+        for a, o, w in zip(names, got, want):
+            if a == "":
+                assert o.output_ids == w.output_ids
+                assert o.output_logprobs == w.output_logprobs
+            else:
+                assert o.output_logprobs != w.output_logprobs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [520, 1300])
+def test_gate_and_up_of_adapters_beside_plain_rows(whole, T):
+    """The three ways through the first half of the MLP: rows without adapter first, last or
+    between, every one as among its like."""
+    from polyrl_amd.rollout.engine import _gate_up
+    e = whole()
+    w = e.model.layers[0].w_gate_up
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(T, w.shape[1], generator=g).bfloat16().cuda()
+    index = torch.randint(-1, 2, (T,), generator=g, dtype=torch.int32).cuda()
+    full = _gate_up(x, w)
+    own = e.model.gate_up_adapted(0, x, index, e.model.adapters.plan(index), 0)
+    some = e.model.gate_up_adapted(0, x, index, e.model.adapters.plan(index), None)
+    has = index >= 0
+    assert torch.equal(some[~has], full[~has]) and torch.equal(some[has], own[has])
+    assert not torch.equal(own[~has], full[~has])
+    order = torch.argsort(has.int(), stable=True)
+    plain = int((~has).sum())
+    x, index = x[order].contiguous(), index[order].contiguous()
+    first = e.model.gate_up_adapted(0, x, index, e.model.adapters.plan(index), plain,
+                                    e.model.adapters.plan(index[plain:]))
+    assert torch.equal(first[:plain], full[order][:plain])
+    # (the product of fewer rows may be another kernel's: a rounding of gate or up, 2^-9 of
+    # them, and one of the result)
+    a, b = first[plain:].float(), own[order][plain:].float()
+    assert ((a - b).abs() <= 0.05 * (b.abs() + 0.1)).all()
 
 
 @pytest.mark.gpu
