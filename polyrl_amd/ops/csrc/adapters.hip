@@ -81,10 +81,10 @@ DEV_INLINE i32x4_t load_some(const T* p, int have) {
 }
 
 // ---------------------------------------------------------------------- plan
-// plan: the number of tiles; for each one (4 ints) its adapter and number of rows; for
-// each one its rows, in places for a whole tile, so that a block knows where to read
-// them before it knows anything else.  Rows without an adapter come last, as tiles of
-// adapter -1.
+// plan: the number of tiles; for each one (4 ints) its adapter, its number of rows and that
+// of the rows of the tiles before it, where its part of h is; for each one its rows, in
+// places for a whole tile, so that a block knows where to read them before it knows anything
+// else.  Rows without an adapter come last, as tiles of adapter -1.
 constexpr int PLAN_HEAD = 4;
 constexpr int MOST_SLOTS = 4095, MOST_RANK = 256;
 
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
                                                             int T, int slots, int tile,
                                                             int most) {
   __shared__ int count[MOST_SLOTS + 1], cursor[MOST_SLOTS + 1];
-  __shared__ int sums[16];
+  __shared__ int sums[2][16];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   for (int s = tid; s <= slots; s += 1024) count[s] = 0;
   __syncthreads();
@@ -145,20 +145,23 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(int* plan, const int
   __syncthreads();
   // each thread a stretch of adapters, then the tiles of the threads before
   const int per = (slots + 1 + 1023) / 1024;
-  int tiles = 0;
-  for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s)
+  int tiles = 0, rows = 0;
+  for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
     tiles += (count[s] + tile - 1) / tile;
-  int n = wave_scan(tiles);
-  if (lane == 63) sums[wid] = n;
+    rows += count[s];
+  }
+  int n = wave_scan(tiles), before = wave_scan(rows);
+  if (lane == 63) sums[0][wid] = n, sums[1][wid] = before;
   __syncthreads();
-  for (int w = 0; w < wid; ++w) n += sums[w];
+  for (int w = 0; w < wid; ++w) n += sums[0][w], before += sums[1][w];
   if (tid == 1023) plan[0] = n;
-  n -= tiles;
+  n -= tiles, before -= rows;
   i32x4_t* entry = reinterpret_cast<i32x4_t*>(plan + PLAN_HEAD);
   for (int s = tid * per; s < min((tid + 1) * per, slots + 1); ++s) {
     cursor[s] = n * tile;
     for (int i = 0; i < count[s]; i += tile, ++n)
-      entry[n] = i32x4_t{s < slots ? s : -1, min(tile, count[s] - i), 0, 0};
+      entry[n] = i32x4_t{s < slots ? s : -1, min(tile, count[s] - i), before + i, 0};
+    before += count[s];
   }
   __syncthreads();
   int* order = plan + PLAN_HEAD + 4 * most;
@@ -176,7 +179,6 @@ struct Shape {
   int T, K, N, parts, rank, rank16;   // rank16: rank rounded up to whole tiles of 16
   long ldx, ldy, ldo;
   int split, most;                    // shares of the inner dimension; places for tiles
-  int places;                         // most times the rows of a tile
   int first[9];                       // columns of the parts
 };
 
@@ -213,7 +215,7 @@ DEV_INLINE void quads_transposed(i32x4_t (&v)[4]) {
   }
 }
 
-// h[share][place][part][j].  A block takes RT * 16 rows of a tile, CT tiles of 16 ranks
+// h[share][row in the tiles' order][part][j].  A block takes RT * 16 rows of a tile, CT tiles of 16 ranks
 // (tile i: ranks 16 * (i / parts) .. of part i % parts) and a share of the inner
 // dimension, each of its NW waves a part of that
 template <typename T, int NW, int RT, int CT, bool WORDS>
@@ -315,13 +317,13 @@ __global__ __launch_bounds__(NW * 64) void adapter_down_kernel(
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += red[w * RT * CT * 256 + o];
-    h[(((long)share * z.places + place + r * 16 + o % 256 / 16) * z.parts + i % z.parts) *
-          z.rank16 + j] = v;
+    h[(((long)share * z.T + t[2] + at % subs * RT * 16 + r * 16 + o % 256 / 16) * z.parts +
+       i % z.parts) * z.rank16 + j] = v;
   }
 }
 
 // ------------------------------------------------------------------------ up
-// h's numbers j .. j + 4 of a place, times s (the shares' sums in their order, zeros from rank
+// h's numbers j .. j + 4 of a row, times s (the shares' sums in their order, zeros from rank
 // on), as PARTS numbers of type T whose sum they are: of bf16 each the upper 8 bits of what
 // those before it leave, cut and not rounded, so that none is larger than h
 template <typename T> constexpr int PARTS = sizeof(T) == 2 ? 3 : 1;
@@ -436,8 +438,8 @@ __global__ __launch_bounds__(256) void adapter_up_few_kernel(
     const int r = threadIdx.x / 16, j = threadIdx.x % 16 * 4;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     if (r < rows && j0 + j < rank)
-      v = shares_sum(h + (((long)place + r) * z.parts + at.part) * z.rank16 + j0 + j,
-                     (long)z.places * z.parts * z.rank16, z.split);
+      v = shares_sum(h + (((long)t[2] + r) * z.parts + at.part) * z.rank16 + j0 + j,
+                     (long)z.T * z.parts * z.rank16, z.split);
     const Four<T> f(v, s, rank - j0 - j);
 #pragma unroll
     for (int p = 0; p < PARTS<T>; ++p) f.put(p, &hs[p][r][j]);
@@ -516,9 +518,9 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
   for (int i = 0; i < 4; ++i) row[i] = mine + i < rows ? own[i] : some;
   constexpr int NB = COLS * GRAN / 256;           // words of b that a thread brings
   constexpr int NH = 64 * PRE / 4 / 256;
-  const long share = (long)z.places * z.parts * z.rank16;
+  const long share = (long)z.T * z.parts * z.rank16;
   const T* bb = b + ((long)max(slot, 0) * z.N + n0) * z.rank;
-  const float* hh = h + ((long)place * z.parts + at.part) * z.rank16;
+  const float* hh = h + ((long)t[2] * z.parts + at.part) * z.rank16;
   i32x4_t bv[NB];
   f32x4_t hv[NH];
   auto fetch = [&](int j0) {
@@ -658,7 +660,7 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
   z.split = (int)std::max<long>(
       1, std::min<long>({512 / blocks, (long)z.K * y.element_size() / (NW * 256),
                          MOST_SPLIT}));
-  auto h = torch::empty({(long)z.split * z.places * z.parts * z.rank16},
+  auto h = torch::empty({(long)z.split * z.T * z.parts * z.rank16},
                         y.options().dtype(torch::kFloat32));
   TORCH_CHECK(blocks * z.split < (1L << 31), "adapter_add: too many rows");
   auto down = [&](auto kern, int waves) {
@@ -746,7 +748,6 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
   z.rank = (int)r, z.rank16 = (int)((r + 15) / 16 * 16);
   z.ldx = x.stride(0), z.ldy = y.stride(0), z.ldo = out.stride(0);
   z.most = (int)most_tiles(T, S);
-  z.places = z.most * tile_rows(T);
   TORCH_CHECK(plan.device() == y.device() && plan.scalar_type() == torch::kInt32 &&
                   rows == T && plan.numel() == PLAN_HEAD + (4L + tile_rows(T)) * z.most,
               "adapter_add: a plan of other rows");

@@ -196,6 +196,25 @@ def test_many_rows_and_slots():
 
 
 @pytest.mark.gpu
+def test_work_space_is_the_rows():
+    """Of many adapters most tiles are of few rows: what lies between the two products
+    takes rows * parts * rank numbers of 32 bits, up to four shares of them, and not the
+    places of tiles."""
+    T, K, widths, r, S = 2000, 8, (8, 8, 8), 256, 4095
+    y, x, a, b, scale = make("cuda", BF16, T, K, widths, r, S)
+    index = torch.randperm(S, generator=torch.Generator().manual_seed(3))[:T].int()
+    plan = ops.adapter_plan(index.cuda(), S)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = ops.adapter_add(y, x, a, b, scale, plan, widths)
+    most = torch.cuda.max_memory_allocated() - before
+    assert most <= 4 * T * len(widths) * r * 4 + 2 * y.numel() * 2 + (1 << 21)
+    want, size = expected(y, x, a, b, scale, index, widths)
+    close(got, want, size, y, K, r)
+
+
+@pytest.mark.gpu
 def test_result_does_not_hang_on_the_order_of_rows():
     T, K, widths, r, S = 600, 512, (96,), 24, 4
     y, x, a, b, scale = make("cuda", BF16, T, K, widths, r, S)
