@@ -610,7 +610,12 @@ __global__ __launch_bounds__(256, PRE == 32 ? 4 : 3) void adapter_up_kernel(
 }
 
 // ------------------------------------------------------------------ bindings
-// rows of a tile: 16 of few rows, whose tiles would stay empty
+// Rows of a tile: 16 of few rows, whose tiles would stay empty.  By rows alone: the rows of
+// each adapter, which decide, are known on the device.  (us, 4096 -> 4096, 1024, 1024 bf16,
+// rank 16, tiles of 16 and of 64: 4 adapters, 48, 128, 256, 257, 512, 1024 rows 9.8, 10.1, 10.7,
+// 10.6, 12.4, 18.2 and 10.0, 10.2, 10.9, 11.0, 12.4, 16.1; 64 adapters 15.0, 17.8, 18.5, 18.4,
+// 19.6, 21.5 and 25.8, 32.0, 33.2, 33.0, 34.6, 38.7; 512 adapters 15.0, 25.4, 50, 56, 93, 94 and
+// 25.5, 53.6, 113, 116, 217, 225.  So beyond the line many adapters would do better in 16.)
 static int tile_rows(long T) { return T <= 256 ? 16 : 64; }
 static long most_tiles(long T, long slots) {
   return T / tile_rows(T) + std::min(T, slots + 1);
@@ -645,7 +650,10 @@ static void launch_adapter_add(torch::Tensor& out, const torch::Tensor& y,
   // are too few blocks otherwise, of many each one reads A again (620 rows, fp32, 8960 -> 20
   // 21 us in blocks of 32 rows and 16 of 16; 6504 rows, bf16, 14336 -> 32, before the
   // loads were dealt as they are, 72 and 97; since then, four projections of those rows, 132
-  // in blocks of 8 waves and 125 of 4).
+  // in blocks of 8 waves and 125 of 4).  Around the line, both products, as at tile_rows:
+  // 4 adapters, 512, 1024, 1500, 2048, 4096 rows 12.4, 16.2, 23.3, 23.3, 38.8 in blocks of 16
+  // rows and 15.1, 18.4, 23.2, 26.8, 38.2 of 32; 64 adapters 34.7, 38.1, 40.9, 42.2, 52.9 and
+  // 25.1, 26.8, 29.2, 31.0, 39.3.
   const int sixteens = tile_rows(z.T) / 16, RT = z.T <= 1024 ? 1 : 2, NW = RT == 1 ? 16 : 4;
   const int subs = sixteens / RT;
   // Tiles of ranks that a block takes: all of them in equal groups, of up to two where a wave
