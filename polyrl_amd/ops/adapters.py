@@ -65,7 +65,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor,
             () if widths is None else widths, out)
     widths = [y.shape[1]] if widths is None else [int(w) for w in widths]
     if torch.is_grad_enabled() and any(
-            t.requires_grad for t in (y, x, a, b, scale)):
+            t is not None and t.requires_grad for t in (y, x, a, b, scale, out)):
         raise RuntimeError("adapter_add has no gradients: call it under "
                            "torch.no_grad()")
     if plan.rows != y.shape[0] or a.shape[0] != plan.slots:

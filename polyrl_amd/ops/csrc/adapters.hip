@@ -715,7 +715,8 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                           const c10::optional<torch::Tensor>& into) {
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(y.requires_grad() || x.requires_grad() || a.requires_grad() ||
-                    b.requires_grad() || scale.requires_grad()),
+                    b.requires_grad() || scale.requires_grad() ||
+                    (into.has_value() && into->requires_grad())),
               "adapter_add has no gradients: call it under torch.no_grad()");
   torch::Tensor out = into.has_value() ? *into : torch::empty(y.sizes(), y.options());
   if (widths.empty() && y.dim() == 2) widths.push_back(y.size(1));
@@ -785,5 +786,6 @@ torch::Tensor adapter_add(const torch::Tensor& y, const torch::Tensor& x,
                        words_out);
   else
     TORCH_CHECK(false, "adapter_add: dtype must be bf16 or fp32");
+  if (into.has_value()) written(out);
   return out;
 }

@@ -311,6 +311,7 @@ void adjust_logits(torch::Tensor out, torch::Tensor logits, torch::Tensor rows,
   else if (logits.scalar_type() == torch::kFloat32) go(float{});
   else TORCH_CHECK(false, "adjust_logits: dtype must be bf16 or fp32");
   HIP_CHECK_KERNEL();
+  written(out);
 }
 
 void append_tokens(torch::Tensor history, torch::Tensor total_len, torch::Tensor rows,

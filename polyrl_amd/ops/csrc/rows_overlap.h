@@ -6,6 +6,11 @@
 
 #include <algorithm>
 
+// An operand that a kernel has written: what autograd saved of it is not it any more
+inline void written(const torch::Tensor& out) {
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // a, b: rows of adjacent numbers (N, W) that may lie apart, or contiguous tensors.  Exact:
 // rows of one between those of the other, columns beside its columns, do not overlap.
 inline bool rows_overlap(const torch::Tensor& a, const torch::Tensor& b) {

@@ -155,7 +155,8 @@ def adjust_logits(logits: torch.Tensor, rules: LogitRules, rows: torch.Tensor,
         raise ValueError(f"adjust_logits: logits (N, {rules.vocab})")
     if rows.dtype != torch.int32 or rows.shape != logits.shape[:1]:
         raise ValueError("adjust_logits: rows (N,) int32")
-    if logits.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (
+            logits.requires_grad or out is not None and out.requires_grad):
         raise RuntimeError("adjust_logits has no gradients: call it under "
                            "torch.no_grad()")
     if logits.is_cuda:

@@ -341,6 +341,31 @@ def test_outputs_on_top_of_operands(dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_outputs_that_autograd_knows(dev):
+    """An output with a gradient of its own is refused; one that a backward pass still needs
+    is found changed there, as with any operator in place."""
+    y, x, a, b, scale = make(dev, F32, 6, 32, (16,), 8, 2)
+    plan = ops.adapter_plan(torch.zeros(6, dtype=torch.int32, device=dev), 2)
+    leaf = torch.zeros(6, 16, device=dev, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError):
+            ops.adapter_add(y, x, a, b, scale, plan, out=out)
+        with torch.no_grad():
+            ops.adapter_add(y, x, a, b, scale, plan, out=out)
+    w = torch.ones(16, 3, device=dev, requires_grad=True)
+    for out in (torch.zeros_like(y), y):
+        loss = (out @ w).sum()
+        ops.adapter_add(y, x, a, b, scale, plan, out=out)
+        with pytest.raises(RuntimeError):
+            loss.backward()
+    with torch.inference_mode():
+        z = y.clone()
+    ops.adapter_add(z, x, a, b, scale, plan) # (tensors of inference have no versions)
+    with torch.inference_mode():
+        ops.adapter_add(z, x, a, b, scale, plan, out=z)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_refusals(dev):
     y, x, a, b, scale = make(dev, BF16, 6, 32, (16,), 8, 2)
     index = torch.zeros(6, dtype=torch.int32, device=dev)

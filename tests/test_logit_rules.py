@@ -291,6 +291,33 @@ def test_outputs_on_top_of_logits(dev, dtype):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+def test_outputs_that_autograd_knows(dev):
+    """An output with a gradient of its own is refused; one that a backward pass still needs
+    is found changed there, as with any operator in place."""
+    rules = ops.LogitRules(1, 40, 6, dev)
+    rules.set(0, allowed=[3])
+    rows = torch.zeros(2, dtype=torch.int32, device=dev)
+    logits = torch.zeros(2, 40, device=dev)
+    leaf = torch.zeros(2, 40, device=dev, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError):
+            ops.adjust_logits(logits, rules, rows, out=out)
+        with torch.no_grad():
+            ops.adjust_logits(logits, rules, rows, out=out)
+    w = torch.ones(40, 3, device=dev, requires_grad=True)
+    for out in (torch.zeros_like(logits), logits):
+        loss = (out @ w).sum()
+        ops.adjust_logits(logits, rules, rows, out=out)
+        with pytest.raises(RuntimeError):
+            loss.backward()
+    with torch.inference_mode():
+        z = logits.clone()
+    ops.adjust_logits(z, rules, rows)
+    with torch.inference_mode():
+        ops.adjust_logits(z, rules, rows, out=z)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_refusals(dev):
     rules = ops.LogitRules(2, 40, 6, dev, biases=1)
     for kw in (dict(repetition=0.0), dict(repetition=-1.0),
