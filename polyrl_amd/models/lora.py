@@ -48,6 +48,8 @@ class LoRALinear(nn.Module):
         super().__init__()
         if dropout > 0 and seeded_dropout > 0:
             raise ValueError("one kind of dropout")
+        if not 0.0 <= seeded_dropout <= 1.0:
+            raise ValueError(f"dropout {seeded_dropout}")
         self.base = base
         for p in self.base.parameters():
             p.requires_grad_(False)

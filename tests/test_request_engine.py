@@ -618,6 +618,17 @@ def test_dropout_of_lora_refusals():
         export_adapter(lin)
 
 
+def test_dropout_rates_that_are_none():
+    """A negative rate or none at all is refused before the layer is changed."""
+    for p in (-0.1, 1.5, float("nan")):
+        lin = torch.nn.Linear(4, 4)
+        with pytest.raises(ValueError):
+            LoRALinear(lin, 2, seeded_dropout=p)
+        assert lin.weight.requires_grad
+    assert isinstance(LoRALinear(lin, 2, seeded_dropout=0.0).dropout,
+                      torch.nn.Identity)
+
+
 TP_WORKER = r"""
 import sys; sys.path.insert(0, "tests")
 import torch, torch.distributed as dist
