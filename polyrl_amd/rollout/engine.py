@@ -725,12 +725,17 @@ class Engine:
 
     def add_request(self, rid: str, input_ids: List[int],
                     sampling: SamplingParams):
+        self._admit(rid, input_ids, sampling,
+                    self._check_sampling(sampling, input_ids))
+        return rid
+
+    def _admit(self, rid: str, input_ids: List[int], sampling: SamplingParams,
+               words) -> Request:
         assert len(input_ids) > 0
-        words = self._check_sampling(sampling, input_ids)
         req = Request(rid=rid, input_ids=list(input_ids), sampling=sampling,
                       arrival_t=time.time(), first_words=words)
         self.waiting.append(req)
-        return rid
+        return req
 
     def add_request_group(self, rid_prefix: str, input_ids: List[int],
                           sampling: SamplingParams, n: int):
@@ -745,13 +750,10 @@ class Engine:
         words = self._check_sampling(sampling, input_ids)
         if n == 1 or not self.enable_prefix_sharing:
             for s_ in range(n):
-                self.add_request(f"{rid_prefix}-s{s_}", input_ids, sampling)
+                self._admit(f"{rid_prefix}-s{s_}", input_ids, sampling, words)
             return
-        parent = Request(rid=f"{rid_prefix}-s0", input_ids=list(input_ids),
-                         sampling=sampling, arrival_t=time.time(),
-                         first_words=words)
+        parent = self._admit(f"{rid_prefix}-s0", input_ids, sampling, words)
         parent.group_children = [f"{rid_prefix}-s{s_}" for s_ in range(1, n)]
-        self.waiting.append(parent)
 
     def abort_request(self, rid: Optional[str] = None, abort_all: bool = False):
         """Mark requests aborted; they are emitted with partial output on the

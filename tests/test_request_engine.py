@@ -413,6 +413,29 @@ def test_rules_that_32_bits_do_not_hold(models):
     assert out.output_ids == [5] * 4
 
 
+@pytest.mark.parametrize("sharing", [True, False])
+@pytest.mark.parametrize("n", [1, 3])
+def test_groups_are_admitted_whole(models, sharing, n):
+    """One question to a token_mask decides on all samples of a group: none is left behind
+    by a refusal of another."""
+    e = engine(models[0][1])
+    e.enable_prefix_sharing = sharing
+    asked = []
+
+    def mask(out):
+        asked.append(list(out))
+        if len(asked) > 1 and not out:
+            raise KeyError("asked twice")
+        return [7]
+    e.add_request_group("g", PROMPTS[0], greedy(2, token_mask=mask), n)
+    assert asked == [[]]
+    outs = []
+    while e.has_work():
+        outs += e.step()
+    assert sorted(o.rid for o in outs) == [f"g-s{i}" for i in range(n)]
+    assert all(o.output_ids == [7, 7] for o in outs)
+
+
 def test_numbers_that_no_table_holds(models):
     """Token ids beyond 64 bits, numbers beyond floats, a mask that fails at once: the
     request is refused as others are."""
