@@ -14,10 +14,10 @@
 // read A in every block of columns; h is 1% of y.)
 //
 // What bounds it: memory, prompts by y and out (6504 rows, ranks 32, the four projections of
-// 4096 / 6144 / 14336 numbers, 1.43 GB: 370 us, 3.9 TB/s; the widest, 746 MB, 152 us, where a
-// copy of the same tiles takes 131), decode by the adapters (57 rows of as many adapters of
-// ranks 64 and 32, 0.45 GB: 148 us, 3.0 TB/s); one row by nine launches, 34 us in a graph and
-// 43 issued one by one.
+// 4096 / 6144 / 14336 numbers, 1.43 GB: 373 us, 3.8 TB/s; the widest, 746 MB, 152 to 157 us,
+// where a copy of the same tiles takes 131), decode by the adapters (57 rows of as many adapters
+// of ranks 64 and 32, 0.45 GB: 149 us, 3.0 TB/s; a wave of ``down`` has one round of its loads on
+// its way); one row by nine launches, 34 us in a graph and 35 to 45 issued one by one.
 //
 // Matrix cores: 16x16x32 in bf16, 16x16x4 in fp32.  h is a sum in 32 bits; as an operand
 // in bf16 it is cut into three bf16 numbers of 8 bits each, whose sum is h, each with its own

@@ -13,7 +13,8 @@
 // What bounds it: memory, and before it the chain row -> slot -> history -> counts in each
 // block (128 x 128256 bf16, 257 to 512 tokens of history, 16 biases: 17.0 us, 3.9 TB/s, 12
 // without rules; 64 x 151936 fp32 with masks 17.6, 4.5 TB/s, what a copy takes).  Long
-// histories are read by every chunk of their row (33 x 152064, 9000 to 32768 tokens: 18.6).
+// histories are read by every chunk of their row, which waits for each round of them but the
+// first (33 x 152064, 9000 to 32768 tokens: 18.6).
 // What it took: 4-byte reads of the history, one waited for after the other 54 us of the
 // last, words 33; loads of the logits behind those of the history, so that a wait for
 // these does not wait for them, and barriers for LDS alone 19.9 -> 18.1 of the first; blocks of

@@ -625,7 +625,7 @@ class Engine:
         self._graphs: Dict[int, dict] = {}      # batch size -> capture state
         self._graph_pool = None
         self._graph_max_pages = (self.max_model_len + page_size - 1) // page_size
-        # EXPERIMENTAL (round-3 candidate, default OFF): pad the graphed
+        # EXPERIMENTAL (default OFF): pad the graphed
         # decode batch up to a bucket size so EOS-staggered serving (B
         # shrinking every few steps) replays existing captures instead of
         # capturing a fresh graph per exact B.  Dummy rows write KV into a
