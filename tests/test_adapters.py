@@ -321,14 +321,14 @@ def test_outputs_on_top_of_operands(dev):
     y = pool[64:].as_strided((T, N), (40, 1))
     x = pool[1024:1024 + T * K].view(T, K)
     a = pool[2048:2048 + S * r * K].view(S, 1, r, K)
-    b = pool[3072:3072 + S * N * r].view(S, N, r)
+    b = pool[3200:3200 + S * N * r].view(S, N, r)
     scale = torch.ones(S, device=dev)
     index = torch.arange(T, dtype=torch.int32) % (S + 1) - 1
     plan = ops.adapter_plan(index.to(dev), S)
     keep = pool.clone()
     at = lambda first, pitch=40: pool.as_strided((T, N), (pitch, 1), first)
     for out in (at(64 + 40), at(64 - 40), at(64 + 15), at(64 - 1), at(64, 41), at(66, 16),
-                at(1024, N), at(1024 + T * K - 1), at(2048, N), at(3072 + 5, 33)):
+                at(1024, N), at(1024 + T * K - 1), at(2048, N), at(3200 + 5, 33)):
         with pytest.raises((ValueError, RuntimeError)):
             ops.adapter_add(y, x, a, b, scale, plan, out=out)
     assert torch.equal(pool, keep)                # refused before anything is written
